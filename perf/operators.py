@@ -1,0 +1,367 @@
+"""Measured cases of the optimizer operators (dtt.optim): clipping by the global gradient norm, the AdamW step with 32-bit
+moments and the AdamW step with 8-bit moments, each over all tensors of a model at once.
+
+`run` computes them in plain torch operations (own = False) or calls the framework (own = True) on the same state.  The
+tensors of a model are views of one buffer, so the plain form needs no loop over tensors: it treats the buffer as one vector.
+"""
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+BLOCK = 256                      # elements that share the two bases of the 8-bit moments
+LR, BETA1, BETA2, EPS, DECAY = 1e-3, 0.9, 0.999, 1e-8, 1e-2
+STEPS_DONE = 100                 # steps behind the state that a case starts from
+M32 = 0xFFFFFFFF
+
+
+# ------------------------------------------------------------------------------------------------ the models' tensors
+def _residual_shapes(depth):
+    """Trainable tensors of the R-FCN detection + tracking network at 600 px (heads, RPN, stages 2 - 4 of the trunk; the
+    stem, stage 1 and every BatchNorm are frozen): element counts, matrices and vectors."""
+    sizes = [512 * 512 * 9, 512, 24 * 512, 24, 48 * 512, 48, 1519 * 512, 1519, 196 * 512, 196]
+    inner, before = 128, 256
+    for blocks in ((4, 6, 3) if depth == 50 else (4, 23, 3)):
+        for b in range(blocks):
+            sizes += [inner * before, inner * inner * 9, inner * 4 * inner]
+            if b == 0:
+                sizes.append(before * inner * 4)
+            before = inner * 4
+        inner *= 2
+    return sizes + [2048 * 512 * 9, 512, 196 * 1051, 196]
+
+
+def _sizes(case):
+    kind = case["set"]
+    if kind == "heads":          # the 1x1 heads alone (a frozen trunk)
+        return [24 * 512, 24, 48 * 512, 48, 1519 * 512, 1519, 196 * 512, 196, 196 * 1051, 196]
+    if kind in ("res50", "res101"):
+        return _residual_shapes(int(kind[3:]))
+    if kind == "blocks":         # generic layers: four square matrices, two wide ones, six vectors
+        w = case["width"]
+        return ([w * w] * 4 + [4 * w * w] * 2 + [w] * 6) * case["count"]
+    # ragged: `count` tensors, odd sizes spread over their logarithm from 1 to `width`
+    sizes, x = [], case["mix"]
+    for _ in range(case["count"]):
+        x = (x * 1103515245 + 12345) & 0x7FFFFFFF
+        sizes.append(max(1, int(math.exp(x / 0x7FFFFFFF * math.log(case["width"])))))
+    return sizes
+
+
+def listed():
+    return [
+        # the gradients of the 1x1 heads (trunk frozen): the smallest call, a launch's latency counts
+        {"name": "clip heads f32", "op": "clip", "set": "heads", "dtype": "f32", "packed": False, "within": False},
+        # all gradients of the Res-101 network, longer than the limit
+        {"name": "clip res101 f32", "op": "clip", "set": "res101", "dtype": "f32", "packed": False, "within": False},
+        # a large 16-bit model late in training: gradients within the limit, nothing to scale
+        {"name": "clip blocks bf16 within", "op": "clip", "set": "blocks", "width": 2048, "count": 24, "dtype": "bf16",
+         "packed": False, "within": True},
+        # a step of the heads alone: latency
+        {"name": "adamw heads f32", "op": "adamw", "set": "heads", "dtype": "f32", "packed": False, "clip": False},
+        # the training step's update of the Res-101 network, gradients clipped on the way
+        {"name": "adamw res101 f32 clipped", "op": "adamw", "set": "res101", "dtype": "f32", "packed": False, "clip": True},
+        # data parallel: gradients and the rest are neighbours in flat buckets, no view is aligned
+        {"name": "adamw res50 f32 packed", "op": "adamw", "set": "res50", "dtype": "f32", "packed": True, "clip": False},
+        # a large 16-bit model
+        {"name": "adamw blocks bf16", "op": "adamw", "set": "blocks", "width": 2048, "count": 12, "dtype": "bf16",
+         "packed": False, "clip": False},
+        # many small odd tensors
+        {"name": "adamw ragged f16", "op": "adamw", "set": "ragged", "width": 200001, "count": 301, "mix": 7, "dtype": "f16",
+         "packed": True, "clip": True},
+        # the same four for 8-bit moments
+        {"name": "adamw8 heads f32", "op": "adamw8", "set": "heads", "dtype": "f32", "packed": False, "clip": False},
+        {"name": "adamw8 res101 f32", "op": "adamw8", "set": "res101", "dtype": "f32", "packed": False, "clip": False},
+        {"name": "adamw8 blocks bf16", "op": "adamw8", "set": "blocks", "width": 2048, "count": 6, "dtype": "bf16",
+         "packed": False, "clip": False},
+        {"name": "adamw8 ragged f16", "op": "adamw8", "set": "ragged", "width": 200001, "count": 301, "mix": 11, "dtype": "f16",
+         "packed": False, "clip": True},
+    ]
+
+
+def draw(rng):
+    case = {"op": rng.choice(("clip", "adamw", "adamw8")), "dtype": rng.choice(("f32", "f32", "bf16", "f16"))}
+    case["set"] = rng.choice(("heads", "res50", "res101", "blocks", "blocks", "ragged", "ragged"))
+    if case["set"] == "blocks":
+        case["width"] = int(math.exp(rng.uniform(math.log(64), math.log(2048))))
+        case["count"] = rng.randint(1, 6)
+    elif case["set"] == "ragged":
+        case["width"] = int(math.exp(rng.uniform(math.log(1000), math.log(2000000))))
+        case["count"] = rng.randint(3, 400)
+        case["mix"] = rng.randint(1, 1 << 30)
+    case["packed"] = case["op"] != "adamw8" and rng.random() < 0.4
+    if case["op"] == "clip":
+        case["within"] = rng.random() < 0.5
+    else:
+        case["clip"] = rng.random() < 0.5
+    case["limit"] = round(math.exp(rng.uniform(math.log(0.05), math.log(0.5))), 4)   # of the norm of the first gradients
+    return case
+
+
+# ------------------------------------------------------------------------------------------------ state
+def _layout(case):
+    """(element counts, first elements, buffer length, elements of the buffer per tensor)"""
+    sizes = _sizes(case)
+    spans = sizes if case["packed"] else [(n + BLOCK - 1) // BLOCK * BLOCK for n in sizes]
+    starts, at = [], 0
+    for s in spans:
+        starts.append(at)
+        at += s
+    return sizes, starts, at, spans
+
+
+def _views(flat, sizes, starts):
+    return [flat[a:a + n] for a, n in zip(starts, sizes)]
+
+
+def prepare(case, seed):
+    dev = torch.device("cuda")
+    sizes, starts, total, spans = _layout(case)
+    gen = torch.Generator(device=dev).manual_seed(seed)
+    dt = DTYPES[case["dtype"]]
+    lengths = torch.tensor(spans, device=dev)
+    real = torch.zeros(total, dtype=torch.bool, device=dev)          # what belongs to a tensor, not to the gap behind it
+    for a, n in zip(starts, sizes):
+        real[a:a + n] = True
+    # gradients: every tensor has its own scale, elements spread over decades, one in twenty is exactly zero
+    scale = torch.exp(torch.randn(len(sizes), device=dev, generator=gen) * 1.5 - 7.0)
+    scale = torch.repeat_interleave(scale, lengths, output_size=total)
+
+    def noise():
+        return torch.randn(total, device=dev, generator=gen)
+    size = torch.exp(noise()) * scale
+    alive = (torch.rand(total, device=dev, generator=gen) > 0.05) & real
+    g = (size * noise() * alive).to(dt)
+    st = {"case": case, "grad": g, "grads": _views(g, sizes, starts)}
+    norm = float(g.float().square().sum(dtype=torch.float64).sqrt())
+    share = case.get("limit", 0.25)
+    if case["op"] == "clip":
+        st["limit"], st["falls"] = (2.0 * norm, 1.0) if case["within"] else (share * norm, 0.999)
+        return st
+    st["limit"] = share * norm if case["clip"] else None
+    p = (noise() * 0.05 * real).to(dt)
+    m = 0.3 * size * noise() * alive
+    v = (size * (1.0 + 0.2 * noise())).square() * alive
+    steps = torch.full((len(sizes),), float(STEPS_DONE), device=dev)
+    st.update(param=p, params=_views(p, sizes, starts), steps=steps, step_list=list(steps.unbind()),
+              decay=[DECAY if n > 2048 else 0.0 for n in sizes])     # no decay of vectors
+    # what a plain program with one buffer keeps: every element's weight decay (and, below, its tensor and place in it)
+    st["decay_of"] = torch.repeat_interleave(torch.tensor(st["decay"], device=dev), lengths, output_size=total)
+    if case["op"] == "adamw":
+        st.update(m=m, v=v, ms=_views(m, sizes, starts), vs=_views(v, sizes, starts))
+        return st
+    st["seed"], st["tensors"] = int(seed) & M32, len(sizes)
+    st["tensor_of"] = torch.repeat_interleave(torch.arange(len(sizes), device=dev), lengths, output_size=total)
+    st["place"] = torch.arange(total, device=dev) - torch.tensor(starts, device=dev)[st["tensor_of"]]
+    half = torch.full((1,), 1 << 19, device=dev, dtype=torch.int64)
+    cm, cv, bases = _encode(m, v, half, half)
+    firsts = [a // BLOCK for a in starts]
+    counts = [s // BLOCK for s in spans]
+    st.update(cm=cm, cv=cv, bases=bases, cms=_views(cm, sizes, starts), cvs=_views(cv, sizes, starts),
+              base_list=[bases[a:a + n] for a, n in zip(firsts, counts)])
+    mo, vo = (torch.zeros(total, device=dev, dtype=torch.bfloat16) for _ in range(2))
+    st.update(m_out=mo, v_out=vo, m_outs=_views(mo, sizes, starts), v_outs=_views(vo, sizes, starts))
+    return st
+
+
+# ------------------------------------------------------------------------------------------------ plain form
+def _norm_and_factor(g32, limit):
+    norm = (g32 * g32).sum(dtype=torch.float64).sqrt()
+    return norm.float(), torch.clamp(limit / (norm + 1e-6), max=1.0).float()
+
+
+def _limit(st):
+    """The limit of this pass.  A backward pass would bring long gradients again each time; here the buffer stays clipped, so the
+    limit falls by 0.1 % from pass to pass, and every pass has the same work."""
+    limit = st["limit"]
+    st["limit"] = limit * st["falls"]
+    return limit
+
+
+def _update(st, g32, m, v):
+    """New parameters (32 bits), moments and step counts."""
+    steps = st["steps"] + 1.0
+    t = steps[0].double()
+    size = (LR / (1.0 - BETA1 ** t)).float()
+    root = (1.0 / torch.sqrt(1.0 - BETA2 ** t)).float()
+    m = m * BETA1 + g32 * (1.0 - BETA1)
+    v = v * BETA2 + (g32 * g32) * (1.0 - BETA2)
+    p = st["param"].float() * (1.0 - LR * st["decay_of"]) - (m / (torch.sqrt(v) * root + EPS)) * size
+    return p, m, v, steps
+
+
+def _mix(x):
+    x = ((x ^ (x >> 16)) * 0x9E3779B9) & M32
+    x = ((x ^ (x >> 15)) * 0x6A09E667) & M32
+    return x ^ (x >> 16)
+
+
+def _dither(st, steps):
+    """The two rounding terms of every element, of 20 bits each, from the state's seed, the tensor, the step and the element: one
+    hash for eight elements, multiplied by an odd number for each of them; its upper half rounds m, its lower half v."""
+    dev = steps.device
+    key = _mix((st["seed"] + 0x9E3779B9 * torch.arange(1, st["tensors"] + 1, device=dev)) & M32)
+    key = _mix((key + steps.long()) & M32)[st["tensor_of"]]
+    at = st["place"]
+    r = (_mix((at >> 3) ^ key) * (2 * (at & 7) + 1)) & M32
+    return (r >> 16) * 16 + 8, (r & 0xFFFF) * 16 + 8
+
+
+def _encode(m, v, um, uv):
+    """Codes of the moments and the bases of the blocks.  The upper 12 bits of |x| (8 of the exponent, 3 of the mantissa, behind a
+    sign that is 0) number a grid of levels; a code counts them from its block's base, 0 is zero.  m: sign and 7 bits, v: 8 bits."""
+    bits_m, bits_v = m.abs().view(torch.int32).long(), v.view(torch.int32).long()
+    qm, qv = (bits_m + um) >> 20, (bits_v + uv) >> 20
+    bm = torch.clamp(qm.view(-1, BLOCK).amax(1) - 126, min=0)
+    bv = torch.clamp(qv.view(-1, BLOCK).amax(1) - 254, min=0)
+    lm = torch.clamp(qm.view(-1, BLOCK) - bm[:, None], min=0).view(-1)
+    lv = torch.clamp(qv.view(-1, BLOCK) - bv[:, None], min=0).view(-1)
+    lv = torch.maximum(lv, (bits_v > 0).long())                      # a second moment that is not zero does not become zero
+    cm = lm | ((m < 0).long() << 7)
+    return cm.to(torch.uint8), lv.to(torch.uint8), torch.stack((bm, bv), 1).to(torch.int16)
+
+
+def _decode(cm, cv, bases):
+    b = bases.int()
+    lm, lv = (cm & 127).int(), cv.int()
+    am = (lm.view(-1, BLOCK) + b[:, :1]).view(-1) << 20
+    av = (lv.view(-1, BLOCK) + b[:, 1:]).view(-1) << 20
+    m = torch.where(lm > 0, am, torch.zeros_like(am)).view(torch.float32)
+    v = torch.where(lv > 0, av, torch.zeros_like(av)).view(torch.float32)
+    return torch.where(cm > 127, -m, m), v
+
+
+def _plain(st):
+    op = st["case"]["op"]
+    g = st["grad"]
+    g32 = g.float()
+    out = {}
+    if op == "clip":
+        out["norm"], c = _norm_and_factor(g32, _limit(st))
+        st["grad"] = out["grad"] = (g32 * c).to(g.dtype)
+        return out
+    if st["limit"] is not None:
+        out["norm"], c = _norm_and_factor(g32, st["limit"])
+        g32 = g32 * c
+    if op == "adamw":
+        p, st["m"], st["v"], st["steps"] = _update(st, g32, st["m"], st["v"])
+        st["param"] = p.to(g.dtype)
+        out.update(param=st["param"], m=st["m"], v=st["v"], steps=st["steps"])
+        return out
+    m, v = _decode(st["cm"], st["cv"], st["bases"])
+    p, m, v, st["steps"] = _update(st, g32, m, v)
+    st["param"] = p.to(g.dtype)
+    st["cm"], st["cv"], st["bases"] = _encode(m, v, *_dither(st, st["steps"]))
+    m, v = _decode(st["cm"], st["cv"], st["bases"])
+    # (a code's value has four significant bits: 16 of them hold it exactly)
+    out.update(param=st["param"], m=m.to(torch.bfloat16), v=v.to(torch.bfloat16), steps=st["steps"])
+    return out
+
+
+# ------------------------------------------------------------------------------------------------ the framework's form
+def _framework():
+    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "pytorch-detect-to-track_amd")
+    if root not in sys.path:
+        sys.path.insert(0, root)
+    from dtt import optim
+    return optim
+
+
+def _own(st):
+    op = st["case"]["op"]
+    optim = _framework()
+    if op == "clip":
+        norm = optim.clip_grads_(st["grads"], _limit(st))
+        return {"norm": norm, "grad": st["grad"]}
+    if op == "adamw":
+        norm = optim.adamw_(st["params"], st["grads"], st["ms"], st["vs"], st["step_list"], lr=LR, betas=(BETA1, BETA2), eps=EPS,
+                            weight_decay=st["decay"], max_norm=st["limit"])
+        out = {"param": st["param"], "m": st["m"], "v": st["v"], "steps": st["steps"]}
+    else:
+        norm = optim.adamw8_(st["params"], st["grads"], st["cms"], st["cvs"], st["base_list"], st["step_list"], lr=LR,
+                             betas=(BETA1, BETA2), eps=EPS, weight_decay=st["decay"], max_norm=st["limit"], seed=st["seed"])
+        optim.unpack_moments_(st["cms"], st["cvs"], st["base_list"], st["m_outs"], st["v_outs"])
+        out = {"param": st["param"], "m": st["m_out"], "v": st["v_out"], "steps": st["steps"]}
+    if st["limit"] is not None:
+        out["norm"] = norm
+    return out
+
+
+def run(state):
+    return _own(state) if own else _plain(state)
+
+
+def work(case):
+    n = sum(_sizes(case))
+    e = 4 if case["dtype"] == "f32" else 2
+    if case["op"] == "clip":
+        return {"bytes": n * e * (1 if case["within"] else 2), "flops": n * (2 if case["within"] else 3)}
+    if case["op"] == "adamw":
+        return {"bytes": n * (3 * e + 16), "flops": n * (17 if case["clip"] else 14)}
+    # codes and bases read and written, their values as 16-bit numbers written
+    return {"bytes": n * (3 * e + 4 + 8 / BLOCK + 4), "flops": n * (17 if case["clip"] else 14)}
+
+
+# ------------------------------------------------------------------------------------------------ 64 bits
+def exact(case, seed):
+    """The definitions in 64 bits, apart from the plain form: levels by logarithm and floor, not by bits."""
+    st = prepare(case, seed)
+    g = st["grad"].double()
+    out = {}
+    if st["limit"] is not None:
+        norm = torch.linalg.vector_norm(g)
+        out["norm"] = norm
+        g *= min(1.0, st["limit"] / (float(norm) + 1e-6))
+    if case["op"] == "clip":
+        return {"norm": out["norm"], "grad": g}
+    t = STEPS_DONE + 1
+
+    def value(code, base, top):
+        level = code & (top - 1)
+        x = (level.view(-1, BLOCK) + base.long()[:, None]).view(-1)
+        exponent, mantissa = x >> 3, x & 7
+        y = torch.ldexp(1.0 + mantissa.double() / 8, exponent - 127)
+        y = torch.where(exponent == 0, torch.ldexp(mantissa.double() / 8, torch.full_like(exponent, -126)), y)
+        return torch.where(level > 0, y, 0.0)
+
+    def rounded(x, u, levels):
+        """x on the grid of eight levels for each power of two, moved by u of a spacing; what lies `levels` below the block's largest is 0"""
+        e = torch.frexp(x)[1].long() - 1
+        e = torch.clamp(e, min=-126)
+        unit = torch.ldexp(torch.ones_like(x), e - 3)
+        k = torch.floor(x / unit + u)                                # 8 .. 16 for normal numbers
+        y = k * unit
+        e2 = torch.clamp(torch.frexp(y)[1].long() - 1, min=-126)
+        level = torch.where(y > 0, (e2 + 126) * 8 + (y / torch.ldexp(torch.ones_like(x), e2 - 3)).long(), 0)
+        base = torch.clamp(level.view(-1, BLOCK).amax(1) - levels, min=0)
+        return y, level, base
+
+    if case["op"] == "adamw":
+        m, v = st["m"].double(), st["v"].double()
+    else:
+        code = st["cm"].long()
+        m = value(code, st["bases"][:, 0], 128) * torch.where(code > 127, -1.0, 1.0)
+        v = value(st["cv"].long(), st["bases"][:, 1], 256)
+    m = BETA1 * m + (1 - BETA1) * g
+    v = BETA2 * v + (1 - BETA2) * g * g
+    step = m / (v.sqrt() / math.sqrt(1 - BETA2 ** t) + EPS)
+    p = st["param"].double()
+    p -= p * (LR * st["decay_of"].double())
+    p -= LR / (1 - BETA1 ** t) * step
+    out.update(param=p, steps=torch.full_like(st["steps"], t, dtype=torch.float64))
+    if case["op"] == "adamw8":
+        um, uv = _dither(st, st["steps"] + 1.0)
+        y, level, base = rounded(m.abs(), um.double() / (1 << 20), 126)
+        y = torch.where(level.view(-1, BLOCK) > base[:, None], y.view(-1, BLOCK), 0.0).view(-1)
+        y, sign = y, torch.where(m < 0, -1.0, 1.0)
+        z, level, base = rounded(v, uv.double() / (1 << 20), 254)
+        small = value(torch.ones_like(level), base, 256)             # the smallest level that is not zero
+        z = torch.where(level.view(-1, BLOCK) > base[:, None], z.view(-1, BLOCK), 0.0).view(-1)
+        z = torch.where((v > 0) & (z == 0), small, z)
+        m, v = y * sign, z
+    out.update(m=m, v=v)
+    return out
