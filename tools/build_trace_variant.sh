@@ -5,7 +5,7 @@ cd "$(dirname "$0")/../pytorch-detect-to-track_amd/csrc"
 B=/tmp/dtt_build_trace; mkdir -p $B ../../tools/_variants
 for f in $(grep "^SRCS" Makefile | sed 's/SRCS := //'); do
   if [ ! -f $B/${f%.hip}.o ] || [ $f -nt $B/${f%.hip}.o ] || [ "$f" = "proposal.hip" ]; then
-    hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -fhip-fp32-correctly-rounded-divide-sqrt -fno-fast-math \
+    hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -fhip-fp32-correctly-rounded-divide-sqrt -fno-fast-math -Xclang -target-feature -Xclang -packed-fp32-ops \
       -I../../include -DDTT_WG_TRACE ${EXTRA_FLAGS} -c $f -o $B/${f%.hip}.o 2>/dev/null &
   fi
 done

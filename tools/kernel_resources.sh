@@ -7,7 +7,7 @@ echo "# static LDS and occupancy (waves per SIMD) of every kernel in libdtt_hip.
 echo "# PSRoI, NMS, proposal, RoI Align and tube kernels size their LDS at launch (DESIGN.md section 3)."
 printf "%-100s %6s %6s %9s %9s %5s\n" kernel VGPRs AGPRs scratch_B LDS_B occ
 for f in $(grep "^SRCS" Makefile | sed 's/SRCS := //'); do
-  hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -fhip-fp32-correctly-rounded-divide-sqrt -fno-fast-math \
+  hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -fhip-fp32-correctly-rounded-divide-sqrt -fno-fast-math -Xclang -target-feature -Xclang -packed-fp32-ops \
     -I../../include -Rpass-analysis=kernel-resource-usage -c $f -o /dev/null 2>&1 | grep "remark:" | sed 's/ \[-Rpass-analysis=kernel-resource-usage\]//' | awk '
     /Function Name:/ {name=$NF}
     / VGPRs:/ {v=$NF}
