@@ -37,7 +37,8 @@ const char* dtt_last_error(void);
  * Tags -- ops: "corr_fwd_op" (one forward correlation, whatever kernels it takes), "corr_bwd_op" (both gradients of one
  * correlation: band kernel + the streamed launch; phase 2 alone when the op is issued in phases, whose phase 1 is "corr_bwd_band"),
  * "proposal_op" (the proposal layer of all images of a call, "nms_op" inside it: both NMS phases), "anchor_target_op",
- * "rpn_loss" (forward of both RPN losses), "psroi_pm_bwd" (the one-launch PSRoI backward of a map's heads);
+ * "rpn_loss" (forward of both RPN losses), "psroi_pm_bwd" (the one-launch PSRoI backward of a map's heads), "grad_norm",
+ * "grad_scale", "adamw", "adamw8" (all launches of one call);
  * kernels: "corr_nhwc" (corr_wsplit_kernel), "corr_fwd_mfma" /
  * "corr_fwd_reduce" (the NCHW pair), "head_gemm", "rpn_head_gemm", "psroi_pm" (position-major poolings), "psroi_fwd_plane",
  * "nms_mask", "nms_sweep", "proposal_select_sort".  tag = NULL detaches.  Events are hipEvent_t handles owned
@@ -588,6 +589,46 @@ int dtt_tube_link(const float* dets, int det_stride, const int* n, const float* 
                   int frames, int max_dets, int max_tracklets, int max_per_image, float nms_thresh, float* kept_boxes,
                   float* kept_scores, int* kept_n, int* path_idx, float* path_total, int* n_paths, void* workspace,
                   size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------- optimizer operators over many tensors at once
+ * The weight update of a training run (the reference takes torch.optim's: trainval_net.py:288-294).  n tensors per call: every
+ * array is a HOST array of n entries holding device pointers / counts / rates; a tensor is a dense run of numel elements in
+ * memory order (the buffers of one tensor in the same order), at any element-aligned address.  dtype: 0 = fp32, 1 = bf16, 2 = fp16.
+ * n = 0 and empty tensors are allowed.  All state, the step counters among it, is in device memory: a captured call counts on with
+ * every replay.  Buffers that a call writes must not overlap anything else it is given (refused: status 0).
+ *
+ * dtt_grad_norm: out[0] = sqrt(sum of all squares), out[1] = min(1, max_norm / (out[0] + 1e-6)) -- the factor that brings the
+ * gradients to the limit; max_norm = infinity asks for the norm alone (factor 1).  Squares and sums in 64 bits, in a fixed order.
+ * workspace: dtt_grad_norm_workspace_bytes(n, numel) bytes, 8-byte aligned.
+ * dtt_grad_scale: grads *= *factor (device scalar); a factor of 1 leaves them untouched. */
+size_t dtt_grad_norm_workspace_bytes(int n, const long* numel);
+int dtt_grad_norm(int n, const void* const* grads, const long* numel, const int* dtypes, double max_norm, float* out,
+                  void* workspace, size_t workspace_bytes, void* stream);
+int dtt_grad_scale(int n, void* const* grads, const long* numel, const int* dtypes, const float* factor, void* stream);
+/* One AdamW step (decoupled weight decay) of n tensors of one dtype.  Per tensor: t = ++*step;  g *= clip[1] (clip: the two floats
+ * of dtt_grad_norm, or NULL);  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;
+ * p = p (1 - lr decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps).   Moments fp32, arithmetic fp32, factors of
+ * t in 64 bits; p rounded once to its dtype.  lr_device: NULL, or per tensor NULL / a device float that replaces lr[i] (read when the
+ * kernel runs).  skip_nonfinite: a norm clip[0] that is not finite leaves parameters, moments and counters as they were.
+ * workspace: dtt_adamw_workspace_bytes(n), 16-byte aligned. */
+size_t dtt_adamw_workspace_bytes(int n);
+int dtt_adamw_step(int n, int dtype, void* const* params, const void* const* grads, float* const* exp_avgs, float* const* exp_avg_sqs,
+                   const long* numel, float* const* steps, const double* lr, const float* const* lr_device,
+                   const double* weight_decay, double beta1, double beta2, double eps, const float* clip, int skip_nonfinite,
+                   void* workspace, size_t workspace_bytes, void* stream);
+/* The same step with the moments in 8 bits: codes of numel bytes each, and bases, two int16 (m, v) per 256 elements in memory order
+ * (all zero = moments of zero).  A code counts levels of a fixed grid -- eight per power of two, the upper 12 bits of the fp32 --
+ * from its block's base: m sign + 7 bits, v 8 bits; bit 14 of a base: the block holds infinities / NaN, whose code is 127 / 255.
+ * Rounding is dithered (right on average: to the nearest of levels 12.5 % apart, beta2 = 0.999 would never move v) by a hash of seed,
+ * ids[i] (NULL = i), step counter and element: the same inputs give the same codes. */
+int dtt_adamw8_step(int n, int dtype, void* const* params, const void* const* grads, unsigned char* const* exp_avgs,
+                    unsigned char* const* exp_avg_sqs, short* const* bases, const long* numel, float* const* steps,
+                    const double* lr, const float* const* lr_device, const double* weight_decay, const unsigned* ids, unsigned seed,
+                    double beta1, double beta2, double eps, const float* clip, int skip_nonfinite, void* workspace,
+                    size_t workspace_bytes, void* stream);
+/* The values that 8-bit moments stand for, as fp32 (out_dtype 0) or bf16 (1; exact: a value has four significant bits). */
+int dtt_adamw8_unpack(int n, const unsigned char* const* exp_avgs, const unsigned char* const* exp_avg_sqs, const short* const* bases,
+                      const long* numel, int out_dtype, void* const* out_avgs, void* const* out_avg_sqs, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,697 @@
+// Optimizer operators over all tensors of a model at once, gfx950: the global gradient norm and the scaling by it, the AdamW step
+// with 32-bit moments and the AdamW step with moments held in 8 bits.
+//
+// Every entry point takes HOST arrays of n device pointers and element counts.  The pointers ride in the kernel arguments (kMax*
+// tensors per launch, under 4 KiB): nothing is uploaded, nothing is kept between calls, and a captured graph holds them by value.
+// A tensor is a dense run of memory in whatever order its dimensions lie; a workgroup owns one chunk of one tensor and finds it
+// from the prefix sums of the tensors' workgroup counts.  All kernels stream: they are bound by HBM, so what they are measured
+// against is bytes / bandwidth.
+#include <float.h>
+#include <math.h>
+#include <stdlib.h>
+#include <algorithm>
+#include "common.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxNorm = 160;     // tensors per launch: 8 + 8 + 4 + 4 bytes each
+constexpr int kMaxStep = 80;      // 5 * 8 + 4 bytes each
+constexpr int kMaxStep8 = 72;     // 6 * 8 + 4
+constexpr int kMaxPrepare = 96;   // 4 * 8 + 4
+constexpr int kNormWorkgroups = 4096;
+constexpr long kMaxNumel = 1L << 34;   // element / 8 fits the 32-bit hash input; a launch's workgroups (kMaxNumel / 4096 * kMax*) fit an int
+
+enum { kF32 = 0, kBf16 = 1, kF16 = 2 };
+
+// ------------------------------------------------------------------------------------------------ element types
+// Vector accesses at ELEMENT alignment: views of a flat bucket start anywhere, and the memory pipe takes wide accesses at any
+// element boundary (a line that is cut costs a second request, nothing else).
+template <typename T, int N> struct Wide {
+  typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
+
+template <typename T, int N> __device__ __forceinline__ void load_f32(const T* p, float (&x)[N]) {
+  typedef typename Wide<T, N>::type V;
+  const V v = *reinterpret_cast<const V*>(p);
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = (float)v[i];
+}
+template <typename T, int N> __device__ __forceinline__ void store_f32(T* p, const float (&x)[N]) {
+  typedef typename Wide<T, N>::type V;
+  V v;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = (T)x[i];   // round to nearest even
+  *reinterpret_cast<V*>(p) = v;
+}
+
+// index of the tensor that owns this workgroup: block0[0 .. n] are prefix sums in the kernel arguments.  The lanes compare 64
+// entries at a time (one vector load each) instead of walking them by dependent scalar loads.
+__device__ __forceinline__ int owner(const int* block0, int n, int b) {
+  const int lane = threadIdx.x & 63;
+  int i = 0;
+  for (int k = 0; k < n; k += 64) {
+    const bool before = k + lane < n && block0[k + lane] <= b;
+    i += __popcll(__ballot(before));
+  }
+  return __builtin_amdgcn_readfirstlane(i) - 1;
+}
+
+// ------------------------------------------------------------------------------------------------ gradient norm
+// norm = sqrt(sum of all g^2) and the factor min(1, max_norm / (norm + 1e-6)).  Squares and sums in 64 bits: no overflow for any
+// fp32 gradient, and the order of the partial sums (fixed: chunks, then workgroups in index order) does not show in 32 bits.
+struct NormTable {
+  const void* g[kMaxNorm];
+  long numel[kMaxNorm];
+  int block0[kMaxNorm];
+  int dtype[kMaxNorm];
+  long chunk;          // elements per workgroup, a multiple of kThreads * 8
+  int n;
+};
+
+template <typename T, int N> __device__ __forceinline__ double square_sum(const T* g, long e0, long e1) {
+  double acc[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] = 0.0;
+  long e = e0 + (long)threadIdx.x * N;
+  for (; e + N <= e1; e += (long)kThreads * N) {
+    float x[N];
+    load_f32<T, N>(g + e, x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = __builtin_fma((double)x[i], (double)x[i], acc[i]);
+  }
+  for (; e < e1; ++e) {   // at most N - 1 elements, of one thread
+    const double x = (double)(float)g[e];
+    acc[0] = __builtin_fma(x, x, acc[0]);
+  }
+#pragma unroll
+  for (int s = 1; s < N; s *= 2)
+#pragma unroll
+    for (int i = 0; i + s < N; i += 2 * s) acc[i] += acc[i + s];
+  return acc[0];
+}
+
+template <int NW> __device__ __forceinline__ double workgroup_sum(double x) {
+  __shared__ double part[NW];
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) x += __shfl_xor(x, s);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+  __syncthreads();
+  double t = 0.0;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) t += part[i];
+  return t;
+}
+
+__global__ __launch_bounds__(kThreads) void grad_norm_kernel(NormTable tab, double* __restrict__ partial) {
+  const int i = owner(tab.block0, tab.n, blockIdx.x);
+  const long e0 = (long)((int)blockIdx.x - tab.block0[i]) * tab.chunk;
+  const long e1 = e0 + tab.chunk < tab.numel[i] ? e0 + tab.chunk : tab.numel[i];
+  double s;
+  if (tab.dtype[i] == kF32) s = square_sum<float, 4>(static_cast<const float*>(tab.g[i]), e0, e1);
+  else if (tab.dtype[i] == kBf16) s = square_sum<__bf16, 8>(static_cast<const __bf16*>(tab.g[i]), e0, e1);
+  else s = square_sum<_Float16, 8>(static_cast<const _Float16*>(tab.g[i]), e0, e1);
+  s = workgroup_sum<kThreads / 64>(s);
+  if (threadIdx.x == 0) partial[blockIdx.x] = s;
+}
+
+__global__ __launch_bounds__(1024) void grad_norm_finish_kernel(const double* __restrict__ partial, int n, double max_norm,
+                                                                float* __restrict__ out) {
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += 1024) s += partial[i];
+  s = workgroup_sum<16>(s);
+  if (threadIdx.x == 0) {
+    const double norm = sqrt(s);
+    // (an infinite limit asks for the norm alone; a norm that is not a number stays one in the factor, an infinite one gives 0)
+    const double f = max_norm / (norm + 1e-6);
+    out[0] = (float)norm;
+    out[1] = isinf(max_norm) ? 1.f : f < 1.0 || f != f ? (float)f : 1.f;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ scaling
+struct ScaleTable {
+  void* g[kMaxNorm];
+  long numel[kMaxNorm];
+  int block0[kMaxNorm];
+  int dtype[kMaxNorm];
+  long chunk;
+  int n;
+};
+
+template <typename T, int N> __device__ __forceinline__ void scale_run(T* g, long e0, long e1, float f) {
+  long e = e0 + (long)threadIdx.x * N;
+  for (; e + N <= e1; e += (long)kThreads * N) {
+    float x[N];
+    load_f32<T, N>(g + e, x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] *= f;
+    store_f32<T, N>(g + e, x);
+  }
+  for (; e < e1; ++e) g[e] = (T)((float)g[e] * f);
+}
+
+__global__ __launch_bounds__(kThreads) void grad_scale_kernel(ScaleTable tab, const float* __restrict__ factor) {
+  const float f = *factor;
+  if (f == 1.f) return;   // within the limit: the gradients are neither read nor written
+  const int i = owner(tab.block0, tab.n, blockIdx.x);
+  const long e0 = (long)((int)blockIdx.x - tab.block0[i]) * tab.chunk;
+  const long e1 = e0 + tab.chunk < tab.numel[i] ? e0 + tab.chunk : tab.numel[i];
+  if (tab.dtype[i] == kF32) scale_run<float, 4>(static_cast<float*>(tab.g[i]), e0, e1, f);
+  else if (tab.dtype[i] == kBf16) scale_run<__bf16, 8>(static_cast<__bf16*>(tab.g[i]), e0, e1, f);
+  else scale_run<_Float16, 8>(static_cast<_Float16*>(tab.g[i]), e0, e1, f);
+}
+
+// ------------------------------------------------------------------------------------------------ what a step needs per tensor
+// One thread per tensor: t <- t + 1 in the tensor's step counter, and the step's factors in 64 bits, rounded once:
+// keep = 1 - lr * decay, size = lr / (1 - beta1^t), root = 1 / sqrt(1 - beta2^t); for 8-bit moments the key of its rounding terms.
+// The counters live on the device, so a captured step counts on with every replay.
+struct PrepareTable {
+  float* step[kMaxPrepare];
+  double lr[kMaxPrepare];
+  const float* lr_device[kMaxPrepare];   // learning rate in device memory (a schedule under a captured graph), or NULL
+  double decay[kMaxPrepare];
+  unsigned id[kMaxPrepare];
+  double beta1, beta2;
+  unsigned seed;
+  int n;
+};
+struct Factors {
+  float keep, size, root;
+  unsigned key;
+};
+
+__host__ __device__ __forceinline__ unsigned mix32(unsigned x) {   // multiplicative (golden ratio, sqrt 2) with folded shifts
+  x = (x ^ (x >> 16)) * 0x9E3779B9u;
+  x = (x ^ (x >> 15)) * 0x6A09E667u;
+  return x ^ (x >> 16);
+}
+
+__device__ __forceinline__ bool skipped(const float* clip, int skip_nonfinite) {
+  return skip_nonfinite && !isfinite(clip[0]);
+}
+
+__global__ __launch_bounds__(kMaxPrepare) void adamw_prepare_kernel(PrepareTable tab, const float* __restrict__ clip,
+                                                                    int skip_nonfinite, Factors* __restrict__ factors) {
+  const int i = threadIdx.x;
+  if (i >= tab.n || (clip && skipped(clip, skip_nonfinite))) return;
+  const float t = *tab.step[i] + 1.f;   // (exact up to 2^24 steps)
+  *tab.step[i] = t;
+  const double lr = tab.lr_device[i] ? (double)*tab.lr_device[i] : tab.lr[i];
+  Factors f;
+  f.keep = (float)(1.0 - lr * tab.decay[i]);
+  f.size = (float)(lr / (1.0 - pow(tab.beta1, (double)t)));
+  f.root = (float)(1.0 / sqrt(1.0 - pow(tab.beta2, (double)t)));
+  f.key = mix32(mix32(tab.seed + 0x9E3779B9u * (tab.id[i] + 1u)) + (unsigned)t);
+  factors[i] = f;
+}
+
+struct Consts {
+  float beta1, one_beta1, beta2, one_beta2, eps;
+};
+
+// m <- beta1 m + (1 - beta1) g;  v <- beta2 v + (1 - beta2) g^2;  p <- keep p - size * m / (root sqrt(v) + eps)
+__device__ __forceinline__ void adamw_element(float& p, float g, float& m, float& v, const Consts& k, const Factors& f) {
+  m = m * k.beta1 + g * k.one_beta1;
+  v = v * k.beta2 + (g * g) * k.one_beta2;
+  p = p * f.keep - (m / (sqrtf(v) * f.root + k.eps)) * f.size;
+}
+
+// ------------------------------------------------------------------------------------------------ AdamW, 32-bit moments
+struct StepTable {
+  void* p[kMaxStep];
+  const void* g[kMaxStep];
+  float* m[kMaxStep];
+  float* v[kMaxStep];
+  long numel[kMaxStep];
+  int block0[kMaxStep];
+  int n;
+};
+constexpr int kStepElems = kThreads * 16;   // elements per workgroup
+
+template <typename T, int N>
+__global__ __launch_bounds__(kThreads) void adamw_step_kernel(StepTable tab, const Factors* __restrict__ factors,
+                                                              const float* __restrict__ clip, int skip_nonfinite, Consts k) {
+  const int i = owner(tab.block0, tab.n, blockIdx.x);
+  if (clip && skipped(clip, skip_nonfinite)) return;
+  const float c = clip ? clip[1] : 1.f;
+  const Factors f = factors[i];
+  T* p = static_cast<T*>(tab.p[i]);
+  const T* g = static_cast<const T*>(tab.g[i]);
+  float* m = tab.m[i];
+  float* v = tab.v[i];
+  const long numel = tab.numel[i];
+  long e = (long)((int)blockIdx.x - tab.block0[i]) * kStepElems + (long)threadIdx.x * N;
+#pragma unroll
+  for (int u = 0; u < kStepElems / (kThreads * N); ++u, e += kThreads * N) {
+    if (e + N <= numel) {
+      float xp[N], xg[N], xm[N], xv[N];
+      load_f32<T, N>(p + e, xp);
+      load_f32<T, N>(g + e, xg);
+      load_f32<float, N>(m + e, xm);
+      load_f32<float, N>(v + e, xv);
+#pragma unroll
+      for (int j = 0; j < N; ++j) adamw_element(xp[j], xg[j] * c, xm[j], xv[j], k, f);
+      store_f32<T, N>(p + e, xp);
+      store_f32<float, N>(m + e, xm);
+      store_f32<float, N>(v + e, xv);
+    } else {
+      for (long q = e; q < numel && q < e + N; ++q) {
+        float xp = (float)p[q], xm = m[q], xv = v[q];
+        adamw_element(xp, (float)g[q] * c, xm, xv, k, f);
+        p[q] = (T)xp; m[q] = xm; v[q] = xv;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ moments in 8 bits
+// The upper 12 bits of a non-negative fp32 (8 of the exponent, 3 of the mantissa) number a fixed grid of LEVELS, eight for each
+// power of two.  256 elements in memory order share a base per moment; a code counts levels from it, code 0 is zero:
+//   m: sign and 7 bits, levels base + 1 .. base + 126 (15.7 powers of two below the block's largest; what lies lower is 0)
+//   v: 8 bits, levels base + 1 .. base + 254 (31.7 powers of two, the same span in |g|); a v that is not 0 keeps code 1 at least,
+//      for a zero would turn the next m / sqrt(v) into m / eps.
+// Why a fixed grid with dithered rounding: beta2 = 0.999 moves v by 0.1 % a step, the levels are 12.5 % apart, and to the nearest
+// v would never move again.  x + u with u uniform below one spacing, cut off, is right on average; and since the grid does not
+// move with the base, a value that does not change is not rounded again.
+// Infinity and NaN stay in their element: the base counts finite levels only, bit 14 of the base says that the block holds such
+// values, and the top code (127 / 255, which finite values never reach) is NaN there.
+constexpr int kBlock = 256;
+constexpr int kNanFlag = 0x4000;
+constexpr int kInfLevel = 0x7F8;   // level of infinity; NaN lies above
+
+__device__ __forceinline__ float decode_m(unsigned code, int base) {
+  const unsigned level = code & 127u;
+  unsigned bits = level ? (level + (unsigned)(base & 0x3FFF)) << 20 : 0u;
+  if ((base & kNanFlag) && level == 127u) bits = 0x7FC00000u;
+  return __uint_as_float(bits | (code & 128u) << 24);
+}
+__device__ __forceinline__ float decode_v(unsigned code, int base) {
+  unsigned bits = code ? (code + (unsigned)(base & 0x3FFF)) << 20 : 0u;
+  if ((base & kNanFlag) && code == 255u) bits = 0x7FC00000u;
+  return __uint_as_float(bits);
+}
+
+struct Step8Table {
+  void* p[kMaxStep8];
+  const void* g[kMaxStep8];
+  unsigned char* m[kMaxStep8];
+  unsigned char* v[kMaxStep8];
+  short* base[kMaxStep8];   // (blocks, 2)
+  long numel[kMaxStep8];
+  int block0[kMaxStep8];
+  int n;
+};
+constexpr int kStep8Elems = kThreads * 16;   // elements per workgroup: 16 blocks
+
+__device__ __forceinline__ int wave_max(int x) {
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) x = max(x, __shfl_xor(x, s));
+  return x;
+}
+
+// A wave owns a block: four elements per lane.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void adamw8_step_kernel(Step8Table tab, const Factors* __restrict__ factors,
+                                                               const float* __restrict__ clip, int skip_nonfinite, Consts k) {
+  const int i = owner(tab.block0, tab.n, blockIdx.x);
+  if (clip && skipped(clip, skip_nonfinite)) return;
+  const float c = clip ? clip[1] : 1.f;
+  const Factors f = factors[i];
+  T* p = static_cast<T*>(tab.p[i]);
+  const T* g = static_cast<const T*>(tab.g[i]);
+  unsigned char* cm = tab.m[i];
+  unsigned char* cv = tab.v[i];
+  short* base = tab.base[i];
+  const long numel = tab.numel[i];
+  const long first = (long)((int)blockIdx.x - tab.block0[i]) * kStep8Elems;
+  for (int u = 0; u < kStep8Elems / kThreads / 4; ++u) {
+    const long e0 = first + (long)u * kThreads * 4 + (threadIdx.x >> 6) * kBlock;   // the wave's block
+    if (e0 >= numel) return;
+    const long e = e0 + (threadIdx.x & 63) * 4;
+    const int bm = base[(e0 / kBlock) * 2], bv = base[(e0 / kBlock) * 2 + 1];
+    const unsigned h = mix32((unsigned)(e >> 3) ^ f.key);
+    float xm[4], xv[4];
+    int qm[4], qv[4], top_m = 0, top_v = 0;
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      xm[j] = xv[j] = 0.f; qm[j] = qv[j] = 0;
+      if (e + j < numel) {
+        xm[j] = decode_m(cm[e + j], bm);
+        xv[j] = decode_v(cv[e + j], bv);
+        float xp = (float)p[e + j];
+        adamw_element(xp, (float)g[e + j] * c, xm[j], xv[j], k, f);
+        p[e + j] = (T)xp;
+        const unsigned r = h * (2u * (unsigned)((e + j) & 7) + 1u);
+        qm[j] = (int)(((__float_as_uint(xm[j]) & 0x7FFFFFFFu) + (r >> 16) * 16u + 8u) >> 20);
+        qv[j] = (int)(((__float_as_uint(xv[j]) & 0x7FFFFFFFu) + (r & 0xFFFFu) * 16u + 8u) >> 20);
+        odd = odd || qm[j] >= kInfLevel || qv[j] >= kInfLevel;
+        if (qm[j] < kInfLevel) top_m = max(top_m, qm[j]);
+        if (qv[j] < kInfLevel) top_v = max(top_v, qv[j]);
+      }
+    }
+    top_m = max(wave_max(top_m) - 126, 0);
+    top_v = max(wave_max(top_v) - 254, 0);
+    const int flag = __any(odd) ? kNanFlag : 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (e + j < numel) {
+        const int lm = qm[j] >= kInfLevel ? 127 : max(qm[j] - top_m, 0);
+        const int lv = qv[j] >= kInfLevel ? 255 : max(qv[j] - top_v, xv[j] > 0.f ? 1 : 0);
+        cm[e + j] = (unsigned char)(lm | (xm[j] < 0.f ? 128 : 0));
+        cv[e + j] = (unsigned char)lv;
+      }
+    if ((threadIdx.x & 63) == 0) {
+      base[(e0 / kBlock) * 2] = (short)(top_m | flag);
+      base[(e0 / kBlock) * 2 + 1] = (short)(top_v | flag);
+    }
+  }
+}
+
+struct UnpackTable {
+  const unsigned char* m[kMaxStep8];
+  const unsigned char* v[kMaxStep8];
+  const short* base[kMaxStep8];
+  void* out_m[kMaxStep8];
+  void* out_v[kMaxStep8];
+  long numel[kMaxStep8];
+  int block0[kMaxStep8];
+  int n;
+};
+
+template <typename T> __global__ __launch_bounds__(kThreads) void unpack_moments_kernel(UnpackTable tab) {
+  const int i = owner(tab.block0, tab.n, blockIdx.x);
+  const long numel = tab.numel[i];
+  const long first = (long)((int)blockIdx.x - tab.block0[i]) * kStep8Elems;
+  for (int u = 0; u < kStep8Elems / kThreads; ++u) {
+    const long e = first + (long)u * kThreads + threadIdx.x;
+    if (e >= numel) return;
+    static_cast<T*>(tab.out_m[i])[e] = (T)decode_m(tab.m[i][e], tab.base[i][(e / kBlock) * 2]);
+    static_cast<T*>(tab.out_v[i])[e] = (T)decode_v(tab.v[i][e], tab.base[i][(e / kBlock) * 2 + 1]);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+int type_bytes(int dtype) { return dtype == kF32 ? 4 : 2; }
+
+// Buffers that a call writes must not meet anything else that it reads or writes (the same parameter twice, a moment that is a
+// view of another, a shared step counter): the workgroups run in no order.
+struct Spans {
+  struct Span {
+    uintptr_t lo, hi;
+    bool written;
+    bool operator<(const Span& o) const { return lo < o.lo; }
+  };
+  Span* s = nullptr;
+  long n = 0;
+  explicit Spans(long most) { s = static_cast<Span*>(malloc((size_t)(most > 0 ? most : 1) * sizeof(Span))); }
+  ~Spans() { free(s); }
+  Spans(const Spans&) = delete;
+  void add(const void* p, long bytes, bool written) {
+    if (bytes > 0) { s[n].lo = reinterpret_cast<uintptr_t>(p); s[n].hi = s[n].lo + (uintptr_t)bytes; s[n].written = written; ++n; }
+  }
+  bool clash() {
+    std::sort(s, s + n);
+    uintptr_t any = 0, written = 0;
+    for (long i = 0; i < n; ++i) {
+      if (s[i].lo < written || (s[i].written && s[i].lo < any)) return true;
+      if (s[i].hi > any) any = s[i].hi;
+      if (s[i].written && s[i].hi > written) written = s[i].hi;
+    }
+    return false;
+  }
+};
+
+bool aligned_to(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
+
+long norm_chunk(int n, const long* numel) {
+  long total = 0;
+  for (int i = 0; i < n; ++i) total += numel[i];
+  const long unit = kThreads * 8;
+  long chunk = (total / kNormWorkgroups + unit - 1) / unit * unit;
+  return chunk < 2 * unit ? 2 * unit : chunk;
+}
+
+int check_grads(const char* what, int n, const void* const* grads, const long* numel, const int* dtypes) {
+  DTT_REQUIRE(n >= 0 && (n == 0 || (grads && numel && dtypes)), "%s: null pointer", what);
+  for (int i = 0; i < n; ++i) {
+    DTT_REQUIRE(numel[i] >= 0 && numel[i] <= kMaxNumel, "%s: tensor %d: bad element count", what, i);
+    DTT_REQUIRE(dtypes[i] >= kF32 && dtypes[i] <= kF16, "%s: tensor %d: unknown element type %d", what, i, dtypes[i]);
+    DTT_REQUIRE(numel[i] == 0 || (grads[i] && aligned_to(grads[i], type_bytes(dtypes[i]))), "%s: tensor %d: null or unaligned pointer", what, i);
+  }
+  return 1;
+}
+
+}  // namespace
+
+extern "C" size_t dtt_grad_norm_workspace_bytes(int n, const long* numel) {
+  if (n <= 0 || !numel) return sizeof(double);
+  const long chunk = norm_chunk(n, numel);
+  long blocks = 0;
+  for (int i = 0; i < n; ++i) blocks += numel[i] > 0 ? (numel[i] + chunk - 1) / chunk : 0;
+  return (size_t)(blocks > 0 ? blocks : 1) * sizeof(double);
+}
+
+extern "C" int dtt_grad_norm(int n, const void* const* grads, const long* numel, const int* dtypes, double max_norm, float* out,
+                             void* workspace, size_t workspace_bytes, void* stream_) {
+  hipStream_t stream = static_cast<hipStream_t>(stream_);
+  if (!check_grads("grad_norm", n, grads, numel, dtypes)) return 0;
+  DTT_REQUIRE(out && workspace && aligned_to(workspace, 8), "grad_norm: null or unaligned pointer");
+  DTT_REQUIRE(max_norm >= 0.0, "grad_norm: max_norm must not be negative");
+  DTT_REQUIRE(workspace_bytes >= dtt_grad_norm_workspace_bytes(n, numel), "grad_norm: workspace too small");
+  double* partial = static_cast<double*>(workspace);
+  const long chunk = n > 0 ? norm_chunk(n, numel) : 1;
+  dtt_prof_begin("grad_norm", stream);
+  int blocks = 0;
+  NormTable tab;
+  for (int i = 0; i < n;) {
+    tab.n = 0; tab.chunk = chunk;
+    int here = 0;
+    for (; i < n && tab.n < kMaxNorm; ++i) {
+      if (numel[i] == 0) continue;
+      const int j = tab.n++;
+      tab.g[j] = grads[i]; tab.numel[j] = numel[i]; tab.dtype[j] = dtypes[i]; tab.block0[j] = here;
+      here += (int)((numel[i] + chunk - 1) / chunk);
+    }
+    if (here == 0) break;
+    hipLaunchKernelGGL(grad_norm_kernel, dim3((unsigned)here), dim3(kThreads), 0, stream, tab, partial + blocks);
+    DTT_CHECK_LAUNCH("grad_norm_kernel");
+    blocks += here;
+  }
+  hipLaunchKernelGGL(grad_norm_finish_kernel, dim3(1), dim3(1024), 0, stream, partial, blocks, max_norm, out);
+  DTT_CHECK_LAUNCH("grad_norm_finish_kernel");
+  dtt_prof_end("grad_norm", stream);
+  return 1;
+}
+
+extern "C" int dtt_grad_scale(int n, void* const* grads, const long* numel, const int* dtypes, const float* factor, void* stream_) {
+  hipStream_t stream = static_cast<hipStream_t>(stream_);
+  if (!check_grads("grad_scale", n, grads, numel, dtypes)) return 0;
+  DTT_REQUIRE(factor, "grad_scale: null pointer");
+  Spans spans(n);
+  DTT_REQUIRE(spans.s, "grad_scale: out of host memory");
+  for (int i = 0; i < n; ++i) spans.add(grads[i], numel[i] * type_bytes(dtypes[i]), true);
+  DTT_REQUIRE(!spans.clash(), "grad_scale: two gradients share memory");
+  const long chunk = n > 0 ? norm_chunk(n, numel) : 1;
+  dtt_prof_begin("grad_scale", stream);
+  ScaleTable tab;
+  for (int i = 0; i < n;) {
+    tab.n = 0; tab.chunk = chunk;
+    int here = 0;
+    for (; i < n && tab.n < kMaxNorm; ++i) {
+      if (numel[i] == 0) continue;
+      const int j = tab.n++;
+      tab.g[j] = grads[i]; tab.numel[j] = numel[i]; tab.dtype[j] = dtypes[i]; tab.block0[j] = here;
+      here += (int)((numel[i] + chunk - 1) / chunk);
+    }
+    if (here == 0) break;
+    hipLaunchKernelGGL(grad_scale_kernel, dim3((unsigned)here), dim3(kThreads), 0, stream, tab, factor);
+    DTT_CHECK_LAUNCH("grad_scale_kernel");
+  }
+  dtt_prof_end("grad_scale", stream);
+  return 1;
+}
+
+extern "C" size_t dtt_adamw_workspace_bytes(int n) { return (size_t)(n > 0 ? n : 1) * sizeof(Factors); }
+
+namespace {
+
+// what both steps check of their arguments; the buffers' spans are collected for the overlap check
+int check_step(const char* what, int n, int dtype, void* const* params, const void* const* grads, const long* numel, float* const* steps,
+               const double* lr, const double* decay, double beta1, double beta2, double eps, const float* clip, int skip_nonfinite,
+               const void* workspace, size_t workspace_bytes, Spans& spans) {
+  DTT_REQUIRE(n >= 0 && (n == 0 || (params && grads && numel && steps && lr && decay)), "%s: null pointer", what);
+  DTT_REQUIRE(dtype >= kF32 && dtype <= kF16, "%s: unknown element type %d", what, dtype);
+  DTT_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "%s: betas must lie in [0, 1)", what);
+  DTT_REQUIRE(eps >= 0.0, "%s: eps must not be negative", what);
+  DTT_REQUIRE(!skip_nonfinite || clip, "%s: skip_nonfinite needs the gradients' norm", what);
+  DTT_REQUIRE(workspace && aligned_to(workspace, 16) && workspace_bytes >= dtt_adamw_workspace_bytes(n), "%s: workspace too small or unaligned", what);
+  DTT_REQUIRE(spans.s, "%s: out of host memory", what);
+  const int es = type_bytes(dtype);
+  for (int i = 0; i < n; ++i) {
+    DTT_REQUIRE(numel[i] >= 0 && numel[i] <= kMaxNumel, "%s: tensor %d: bad element count", what, i);
+    DTT_REQUIRE(steps[i] && aligned_to(steps[i], 4), "%s: tensor %d: null or unaligned step counter", what, i);
+    DTT_REQUIRE(lr[i] >= 0.0 && decay[i] >= 0.0, "%s: tensor %d: learning rate and weight decay must not be negative", what, i);
+    DTT_REQUIRE(numel[i] == 0 || (params[i] && grads[i] && aligned_to(params[i], es) && aligned_to(grads[i], es)),
+                "%s: tensor %d: null or unaligned pointer", what, i);
+    spans.add(params[i], numel[i] * es, true);
+    spans.add(grads[i], numel[i] * es, false);
+    spans.add(steps[i], 4, true);
+  }
+  return 1;
+}
+
+int prepare(int n, float* const* steps, const double* lr, const float* const* lr_device, const double* decay, const unsigned* ids,
+            unsigned seed, double beta1, double beta2, const float* clip, int skip_nonfinite, Factors* factors, hipStream_t stream) {
+  PrepareTable tab;
+  tab.beta1 = beta1; tab.beta2 = beta2; tab.seed = seed;
+  for (int i0 = 0; i0 < n; i0 += kMaxPrepare) {
+    tab.n = n - i0 < kMaxPrepare ? n - i0 : kMaxPrepare;
+    for (int j = 0; j < tab.n; ++j) {
+      tab.step[j] = steps[i0 + j]; tab.lr[j] = lr[i0 + j]; tab.decay[j] = decay[i0 + j];
+      tab.lr_device[j] = lr_device ? lr_device[i0 + j] : nullptr;
+      tab.id[j] = ids ? ids[i0 + j] : (unsigned)(i0 + j);
+    }
+    hipLaunchKernelGGL(adamw_prepare_kernel, dim3(1), dim3(kMaxPrepare), 0, stream, tab, clip, skip_nonfinite, factors + i0);
+    DTT_CHECK_LAUNCH("adamw_prepare_kernel");
+  }
+  return 1;
+}
+
+Consts consts(double beta1, double beta2, double eps) {
+  Consts k;
+  k.beta1 = (float)beta1; k.one_beta1 = (float)(1.0 - beta1);
+  k.beta2 = (float)beta2; k.one_beta2 = (float)(1.0 - beta2);
+  k.eps = (float)eps;
+  return k;
+}
+
+}  // namespace
+
+extern "C" int dtt_adamw_step(int n, int dtype, void* const* params, const void* const* grads, float* const* exp_avgs,
+                              float* const* exp_avg_sqs, const long* numel, float* const* steps, const double* lr,
+                              const float* const* lr_device, const double* weight_decay, double beta1, double beta2, double eps,
+                              const float* clip, int skip_nonfinite, void* workspace, size_t workspace_bytes, void* stream_) {
+  hipStream_t stream = static_cast<hipStream_t>(stream_);
+  Spans spans(5L * (n > 0 ? n : 0));
+  if (!check_step("adamw", n, dtype, params, grads, numel, steps, lr, weight_decay, beta1, beta2, eps, clip, skip_nonfinite, workspace,
+                  workspace_bytes, spans)) return 0;
+  DTT_REQUIRE(n == 0 || (exp_avgs && exp_avg_sqs), "adamw: null pointer");
+  for (int i = 0; i < n; ++i) {
+    DTT_REQUIRE(numel[i] == 0 || (exp_avgs[i] && exp_avg_sqs[i] && aligned_to(exp_avgs[i], 4) && aligned_to(exp_avg_sqs[i], 4)),
+                "adamw: tensor %d: null or unaligned moment", i);
+    spans.add(exp_avgs[i], numel[i] * 4, true);
+    spans.add(exp_avg_sqs[i], numel[i] * 4, true);
+  }
+  DTT_REQUIRE(!spans.clash(), "adamw: two of the tensors share memory");
+  Factors* factors = static_cast<Factors*>(workspace);
+  const Consts k = consts(beta1, beta2, eps);
+  dtt_prof_begin("adamw", stream);
+  if (!prepare(n, steps, lr, lr_device, weight_decay, nullptr, 0u, beta1, beta2, clip, skip_nonfinite, factors, stream)) return 0;
+  StepTable tab;
+  for (int i0 = 0; i0 < n; i0 += kMaxStep) {
+    tab.n = n - i0 < kMaxStep ? n - i0 : kMaxStep;
+    int blocks = 0;
+    for (int j = 0; j < tab.n; ++j) {
+      const int i = i0 + j;
+      tab.p[j] = params[i]; tab.g[j] = grads[i]; tab.m[j] = exp_avgs[i]; tab.v[j] = exp_avg_sqs[i]; tab.numel[j] = numel[i];
+      tab.block0[j] = blocks;
+      const long nb = (numel[i] + kStepElems - 1) / kStepElems;
+      blocks += (int)nb;
+    }
+    if (blocks == 0) continue;
+    const dim3 grid((unsigned)blocks), wg(kThreads);
+    if (dtype == kF32) hipLaunchKernelGGL((adamw_step_kernel<float, 4>), grid, wg, 0, stream, tab, factors + i0, clip, skip_nonfinite, k);
+    else if (dtype == kBf16) hipLaunchKernelGGL((adamw_step_kernel<__bf16, 8>), grid, wg, 0, stream, tab, factors + i0, clip, skip_nonfinite, k);
+    else hipLaunchKernelGGL((adamw_step_kernel<_Float16, 8>), grid, wg, 0, stream, tab, factors + i0, clip, skip_nonfinite, k);
+    DTT_CHECK_LAUNCH("adamw_step_kernel");
+  }
+  dtt_prof_end("adamw", stream);
+  return 1;
+}
+
+extern "C" int dtt_adamw8_step(int n, int dtype, void* const* params, const void* const* grads, unsigned char* const* exp_avgs,
+                               unsigned char* const* exp_avg_sqs, short* const* bases, const long* numel, float* const* steps,
+                               const double* lr, const float* const* lr_device, const double* weight_decay, const unsigned* ids,
+                               unsigned seed, double beta1, double beta2, double eps, const float* clip, int skip_nonfinite,
+                               void* workspace, size_t workspace_bytes, void* stream_) {
+  hipStream_t stream = static_cast<hipStream_t>(stream_);
+  Spans spans(6L * (n > 0 ? n : 0));
+  if (!check_step("adamw8", n, dtype, params, grads, numel, steps, lr, weight_decay, beta1, beta2, eps, clip, skip_nonfinite, workspace,
+                  workspace_bytes, spans)) return 0;
+  DTT_REQUIRE(n == 0 || (exp_avgs && exp_avg_sqs && bases), "adamw8: null pointer");
+  for (int i = 0; i < n; ++i) {
+    DTT_REQUIRE(numel[i] == 0 || (exp_avgs[i] && exp_avg_sqs[i] && bases[i] && aligned_to(bases[i], 2)),
+                "adamw8: tensor %d: null or unaligned moment", i);
+    spans.add(exp_avgs[i], numel[i], true);
+    spans.add(exp_avg_sqs[i], numel[i], true);
+    spans.add(bases[i], (numel[i] + kBlock - 1) / kBlock * 4, true);
+  }
+  DTT_REQUIRE(!spans.clash(), "adamw8: two of the tensors share memory");
+  Factors* factors = static_cast<Factors*>(workspace);
+  const Consts k = consts(beta1, beta2, eps);
+  dtt_prof_begin("adamw8", stream);
+  if (!prepare(n, steps, lr, lr_device, weight_decay, ids, seed, beta1, beta2, clip, skip_nonfinite, factors, stream)) return 0;
+  Step8Table tab;
+  for (int i0 = 0; i0 < n; i0 += kMaxStep8) {
+    tab.n = n - i0 < kMaxStep8 ? n - i0 : kMaxStep8;
+    int blocks = 0;
+    for (int j = 0; j < tab.n; ++j) {
+      const int i = i0 + j;
+      tab.p[j] = params[i]; tab.g[j] = grads[i]; tab.m[j] = exp_avgs[i]; tab.v[j] = exp_avg_sqs[i]; tab.base[j] = bases[i];
+      tab.numel[j] = numel[i]; tab.block0[j] = blocks;
+      const long nb = (numel[i] + kStep8Elems - 1) / kStep8Elems;
+      blocks += (int)nb;
+    }
+    if (blocks == 0) continue;
+    const dim3 grid((unsigned)blocks), wg(kThreads);
+    if (dtype == kF32) hipLaunchKernelGGL((adamw8_step_kernel<float>), grid, wg, 0, stream, tab, factors + i0, clip, skip_nonfinite, k);
+    else if (dtype == kBf16) hipLaunchKernelGGL((adamw8_step_kernel<__bf16>), grid, wg, 0, stream, tab, factors + i0, clip, skip_nonfinite, k);
+    else hipLaunchKernelGGL((adamw8_step_kernel<_Float16>), grid, wg, 0, stream, tab, factors + i0, clip, skip_nonfinite, k);
+    DTT_CHECK_LAUNCH("adamw8_step_kernel");
+  }
+  dtt_prof_end("adamw8", stream);
+  return 1;
+}
+
+extern "C" int dtt_adamw8_unpack(int n, const unsigned char* const* exp_avgs, const unsigned char* const* exp_avg_sqs,
+                                 const short* const* bases, const long* numel, int out_dtype, void* const* out_avgs,
+                                 void* const* out_avg_sqs, void* stream_) {
+  hipStream_t stream = static_cast<hipStream_t>(stream_);
+  DTT_REQUIRE(n >= 0 && (n == 0 || (exp_avgs && exp_avg_sqs && bases && numel && out_avgs && out_avg_sqs)), "adamw8_unpack: null pointer");
+  DTT_REQUIRE(out_dtype == kF32 || out_dtype == kBf16, "adamw8_unpack: the values come as fp32 or bf16 (fp16 lacks their range)");
+  const int es = type_bytes(out_dtype);
+  Spans spans(5L * (n > 0 ? n : 0));
+  DTT_REQUIRE(spans.s, "adamw8_unpack: out of host memory");
+  for (int i = 0; i < n; ++i) {
+    DTT_REQUIRE(numel[i] >= 0 && numel[i] <= kMaxNumel, "adamw8_unpack: tensor %d: bad element count", i);
+    DTT_REQUIRE(numel[i] == 0 || (exp_avgs[i] && exp_avg_sqs[i] && bases[i] && aligned_to(bases[i], 2) && out_avgs[i] && out_avg_sqs[i] &&
+                                  aligned_to(out_avgs[i], es) && aligned_to(out_avg_sqs[i], es)),
+                "adamw8_unpack: tensor %d: null or unaligned pointer", i);
+    spans.add(exp_avgs[i], numel[i], false);
+    spans.add(exp_avg_sqs[i], numel[i], false);
+    spans.add(bases[i], (numel[i] + kBlock - 1) / kBlock * 4, false);
+    spans.add(out_avgs[i], numel[i] * es, true);
+    spans.add(out_avg_sqs[i], numel[i] * es, true);
+  }
+  DTT_REQUIRE(!spans.clash(), "adamw8_unpack: two of the tensors share memory");
+  UnpackTable tab;
+  for (int i0 = 0; i0 < n; i0 += kMaxStep8) {
+    tab.n = n - i0 < kMaxStep8 ? n - i0 : kMaxStep8;
+    int blocks = 0;
+    for (int j = 0; j < tab.n; ++j) {
+      const int i = i0 + j;
+      tab.m[j] = exp_avgs[i]; tab.v[j] = exp_avg_sqs[i]; tab.base[j] = bases[i]; tab.out_m[j] = out_avgs[i]; tab.out_v[j] = out_avg_sqs[i];
+      tab.numel[j] = numel[i]; tab.block0[j] = blocks;
+      const long nb = (numel[i] + kStep8Elems - 1) / kStep8Elems;
+      blocks += (int)nb;
+    }
+    if (blocks == 0) continue;
+    const dim3 grid((unsigned)blocks), wg(kThreads);
+    if (out_dtype == kF32) hipLaunchKernelGGL((unpack_moments_kernel<float>), grid, wg, 0, stream, tab);
+    else hipLaunchKernelGGL((unpack_moments_kernel<__bf16>), grid, wg, 0, stream, tab);
+    DTT_CHECK_LAUNCH("unpack_moments_kernel");
+  }
+  return 1;
+}

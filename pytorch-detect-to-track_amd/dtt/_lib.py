@@ -18,6 +18,8 @@ _I = ctypes.c_int
 _F = ctypes.c_float
 _L = ctypes.c_long
 _Z = ctypes.c_size_t
+_D = ctypes.c_double
+_U = ctypes.c_uint
 
 # name -> (restype, argtypes); mirrors include/dtt_hip.h one to one
 SIGNATURES = {
@@ -94,6 +96,13 @@ SIGNATURES = {
     "dtt_tube_link": (_I, [_P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P, _P, _P, _P, _P, _P, _P, _Z, _P]),
     "dtt_anchor_target_finish": (_I, [_P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _F, _F, _P, _P, _P, _P, _P]),
     "dtt_anchor_target_device": (_I, [_P, _P, _P, _P] + [_I] * 8 + [_F, _F, _I, _F, _F] + [_P] * 9 + [_P]),
+    "dtt_grad_norm_workspace_bytes": (_Z, [_I, _P]),
+    "dtt_grad_norm": (_I, [_I, _P, _P, _P, _D, _P, _P, _Z, _P]),
+    "dtt_grad_scale": (_I, [_I, _P, _P, _P, _P, _P]),
+    "dtt_adamw_workspace_bytes": (_Z, [_I]),
+    "dtt_adamw_step": (_I, [_I, _I] + [_P] * 9 + [_D, _D, _D, _P, _I, _P, _Z, _P]),
+    "dtt_adamw8_step": (_I, [_I, _I] + [_P] * 11 + [_U, _D, _D, _D, _P, _I, _P, _Z, _P]),
+    "dtt_adamw8_unpack": (_I, [_I] + [_P] * 4 + [_I, _P, _P, _P]),
 }
 
 _lib = None

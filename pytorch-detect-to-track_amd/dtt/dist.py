@@ -262,9 +262,10 @@ def shard_snippets(n_snippets, rank, world):
     return range(start, start + base + (1 if rank < rem else 0))
 
 
-def make_optimizer(model, cfg, lr=None, optimizer="sgd"):
+def make_optimizer(model, cfg, lr=None, optimizer="sgd", max_norm=None):
     """Per-parameter groups of trainval_net.py:280-294: biases get lr*(DOUBLE_BIAS+1) and no weight decay
-    unless BIAS_DECAY."""
+    unless BIAS_DECAY.  "adamw" / "adamw8" (moments in 32 / 8 bits): dtt.optim.GroupedAdamW, which applies max_norm inside its
+    step; with the others the caller clips (dtt.optim.clip_grad_norm_)."""
     T = cfg.TRAIN
     lr = T.LEARNING_RATE if lr is None else lr
     groups, seen = [], set()
@@ -280,6 +281,9 @@ def make_optimizer(model, cfg, lr=None, optimizer="sgd"):
     if optimizer == "adam":
         # the reference scales only the lr it PRINTS by 0.1 (trainval_net.py:290-292); the groups keep the full rate
         return torch.optim.Adam(groups)
+    if optimizer in ("adamw", "adamw8"):
+        from .optim import GroupedAdamW
+        return GroupedAdamW(groups, state_bits=8 if optimizer == "adamw8" else 32, max_norm=max_norm)
     return GroupedSGD(groups, momentum=T.MOMENTUM)
 
 

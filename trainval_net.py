@@ -44,7 +44,7 @@ def parse_args(argv=None):
     p.add_argument("--bs", dest="batch_size", default=1, type=int)
     p.add_argument("--cag", dest="class_agnostic", action="store_true")
     p.add_argument("--use_det", dest="use_det", action="store_true")
-    p.add_argument("--o", dest="optimizer", default="sgd", type=str)
+    p.add_argument("--o", dest="optimizer", default="sgd", type=str, help="sgd, adam, adamw or adamw8 (moments in 8 bits)")
     p.add_argument("--lr", dest="lr", default=0.001, type=float)
     p.add_argument("--lr_decay_step", dest="lr_decay_step", default=5, type=int)
     p.add_argument("--lr_decay_gamma", dest="lr_decay_gamma", default=0.1, type=float)
@@ -54,6 +54,7 @@ def parse_args(argv=None):
     p.add_argument("--checkepoch", dest="checkepoch", default=1, type=int)
     p.add_argument("--checkpoint", dest="checkpoint", default=0, type=int)
     p.add_argument("--use_tfboard", dest="use_tfboard", default=False, type=bool)
+    p.add_argument("--clip_grad", default=0.0, type=float, help="limit on the norm of all gradients (0: none)")
     # additions for the synthetic loader
     p.add_argument("--iters_per_epoch", default=100, type=int)
     p.add_argument("--height", default=600, type=int)
@@ -115,6 +116,7 @@ def main(argv=None):
     args = parse_args(argv)
     from dtt.config import apply_dataset_defaults, cfg, cfg_from_file
     from dtt.dist import make_optimizer
+    from dtt.optim import GroupedAdamW, clip_grad_norm_
     from dtt.synth import build_model, calibrate_batchnorm_, make_batch
 
     world = int(os.environ.get("WORLD_SIZE", "1"))
@@ -151,7 +153,8 @@ def main(argv=None):
                         pretrained_rfcn=init == "reference" and args.net == "res101").to(dev)
     output_dir = os.path.join(args.save_dir, args.net, args.dataset)
     os.makedirs(output_dir, exist_ok=True)
-    optimizer = make_optimizer(model, cfg, lr=args.lr, optimizer=args.optimizer)
+    optimizer = make_optimizer(model, cfg, lr=args.lr, optimizer=args.optimizer, max_norm=args.clip_grad or None)
+    clip = args.clip_grad and not isinstance(optimizer, GroupedAdamW)   # (that one clips inside its step)
     lr = args.lr * (0.1 if args.optimizer == "adam" else 1.0)
     if args.resume:
         load_name = os.path.join(output_dir, "rfcn_detect_track_{}_{}_{}.pth".format(args.checksession, args.checkepoch,
@@ -232,6 +235,8 @@ def main(argv=None):
                     raise ValueError("bg_num_rois = 0 and fg_num_rois = 0, this should not happen!")
                 loss.backward()
                 runner.finish_gradients()
+            if clip:
+                clip_grad_norm_(model.parameters(), args.clip_grad)
             optimizer.step()
             loss_temp += loss_value
             if (step + 1) % args.disp_interval == 0 and rank == 0:
