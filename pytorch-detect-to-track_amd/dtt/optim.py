@@ -11,8 +11,8 @@ Nothing here waits for the GPU: norms, step counters and the decision to skip a 
 captured into a graph and counts on with every replay.  A captured call keeps the addresses of the tensors it was given and a
 learning rate given as a number; a schedule under a graph passes the rate as a float32 tensor and writes to it.
 """
-import ctypes
 import math
+from array import array
 
 import torch
 
@@ -20,50 +20,77 @@ from . import _lib
 from ._lib import check, ptr, stream_ptr
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_UINT8, _INT16 = 3, 4
 BLOCK = 256                      # elements, in memory order, that share a base of the 8-bit moments
 _NAN_FLAG = 0x4000
+_ONE = (1).to_bytes(8, "little")
+
+_host = None
 
 
-# ------------------------------------------------------------------------------------------------ argument checks
+def _tensorlist():
+    """The compiled module that reads lists of tensors (csrc/tensorlist.cpp)."""
+    global _host
+    if _host is None:
+        try:
+            from . import _tensorlist as module
+        except ImportError as e:
+            raise _lib.DttLibraryError("dtt/_tensorlist.so is missing or does not load (%s) -- build it with `make -C %s` (or "
+                                       "__graft_entry__.build())" % (e, _lib.CSRC))
+        _host = module
+    return _host
+
+
+# ------------------------------------------------------------------------------------------------ lists of tensors
+class _List:
+    """Addresses, element counts and types (as the arrays that the library takes) of a list of tensors."""
+    __slots__ = ("tensors", "ptrs", "counts", "types", "device", "type", "odd")
+
+    def __init__(self, what, tensors):
+        self.tensors = tensors
+        try:
+            self.ptrs, self.counts, self.types, self.device, self.type, self.odd = _tensorlist().describe(tensors)
+        except TypeError as e:
+            raise TypeError("%s: %s" % (what, e)) from None
+
+    def __len__(self):
+        return len(self.tensors)
+
+    def floats(self, what, name):
+        """All strided float32, bfloat16 or float16."""
+        if not 0 <= self.type <= 2:
+            for t in self.tensors:
+                if t.layout != torch.strided or t.dtype not in _DTYPES:
+                    raise TypeError("%s: %s must be dense float32, bfloat16 or float16 tensors (got %s, %s)" % (what, name, t.dtype, t.layout))
+        return self
+
+    def dense(self, what, name):
+        if self.odd >= 0:
+            t = self.tensors[self.odd]
+            raise ValueError("%s: %s must be dense (entry %d: shape %s, strides %s)" % (what, name, self.odd, tuple(t.shape), t.stride()))
+        return self
+
+
+def _device_of(what, lists):
+    """The one device of all tensors, as an index."""
+    dev = lists[0].device
+    for x in lists:
+        if x.device == -1 or (x.device == -2 and not all(t.is_cuda for t in x.tensors)):
+            raise RuntimeError("dtt ops run on the GPU only (%s got a %s tensor); there is no CPU fallback" %
+                               (what, next(t.device for t in x.tensors if not t.is_cuda)))
+    if dev == -2 or any(x.device != dev for x in lists):
+        raise ValueError("%s: all tensors must be on one device (got %s)" % (what, sorted({str(t.device) for x in lists for t in x.tensors})))
+    return dev
+
+
 def _dense(t):
     """Whether t fills one run of memory, in whatever order of its dimensions."""
-    if t.is_contiguous():
-        return True
-    expected = 1
-    for stride, size in sorted((st, sz) for sz, st in zip(t.shape, t.stride()) if sz != 1):
-        if stride != expected:
-            return False
-        expected *= size
-    return True
+    return t.is_contiguous() or _tensorlist().describe([t])[5] < 0
 
 
 def _same_order(a, b):
     """Whether a and b (same shape, a dense) hold the same element at the same place of their memory."""
     return (a.is_contiguous() and b.is_contiguous()) or all(sz == 1 or x == y for sz, x, y in zip(a.shape, a.stride(), b.stride()))
-
-
-def _device_of(what, tensors):
-    """The one device of all tensors, as an index."""
-    dev = None
-    for t in tensors:
-        if not isinstance(t, torch.Tensor):
-            raise TypeError("%s: expected tensors (got %s)" % (what, type(t).__name__))
-        d = t.get_device()
-        if d < 0:
-            raise RuntimeError("dtt ops run on the GPU only (%s got a %s tensor); there is no CPU fallback" % (what, t.device))
-        if dev is None:
-            dev = d
-        elif d != dev:
-            raise ValueError("%s: all tensors must be on one device (got cuda:%d and cuda:%d)" % (what, dev, d))
-    return dev
-
-
-def _check_gradients(what, grads):
-    grads = list(grads)
-    for g in grads:
-        if isinstance(g, torch.Tensor) and (g.layout != torch.strided or g.dtype not in _DTYPES):
-            raise TypeError("%s: gradients must be dense float32, bfloat16 or float16 tensors (got %s, %s)" % (what, g.dtype, g.layout))
-    return grads, _device_of(what, grads)
 
 
 def _limit(what, max_norm):
@@ -73,48 +100,38 @@ def _limit(what, max_norm):
     return max_norm
 
 
-def _pointers(tensors):
-    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
-
-
-def _longs(values):
-    return (ctypes.c_long * len(values))(*values)
-
-
-def _written(tensors):
+def _written(*lists):
     """The kernels write behind autograd's back: tell it, as torch's own in-place operations do."""
-    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+    for x in lists:
+        _tensorlist().bump(x)
 
 
 # ------------------------------------------------------------------------------------------------ gradient norm
-def _norm_and_factor(grads, max_norm, dev):
-    """(2,) float32: the norm of all gradients and the factor min(1, max_norm / (norm + 1e-6))."""
+def _norm_and_factor(grads, max_norm):
+    """(2,) float32: the norm of all gradients (a _List on one GPU) and the factor min(1, max_norm / (norm + 1e-6))."""
     n = len(grads)
-    out = torch.empty(2, dtype=torch.float32, device=grads[0].device)
-    numel = _longs([g.numel() for g in grads])
+    device = grads.tensors[0].device
+    out = torch.empty(2, dtype=torch.float32, device=device)
     L = _lib.lib()
-    with torch.cuda.device(dev):
-        nbytes = L.dtt_grad_norm_workspace_bytes(n, numel)
-        ws = torch.empty(nbytes // 8, dtype=torch.float64, device=out.device)
-        check(L.dtt_grad_norm(n, _pointers(grads), numel, (ctypes.c_int * n)(*[_DTYPES[g.dtype] for g in grads]), max_norm, ptr(out), ptr(ws),
-                              nbytes, stream_ptr(dev)), "grad_norm")
+    with torch.cuda.device(device):
+        nbytes = L.dtt_grad_norm_workspace_bytes(n, grads.counts)
+        ws = torch.empty(nbytes // 8, dtype=torch.float64, device=device)
+        check(L.dtt_grad_norm(n, grads.ptrs, grads.counts, grads.types, max_norm, ptr(out), ptr(ws), nbytes, stream_ptr(device)), "grad_norm")
     return out
 
 
-def _any_order(what, grads):
-    for i, g in enumerate(grads):
-        if not _dense(g):
-            raise ValueError("%s: gradient %d is not dense (shape %s, strides %s)" % (what, i, tuple(g.shape), g.stride()))
+def _gradients(what, grads):
+    grads = _List(what, list(grads)).floats(what, "gradients")
+    if len(grads):
+        _device_of(what, [grads])
+    return grads.dense(what, "gradients")
 
 
 @torch.no_grad()
 def grad_norm(grads):
     """The 2-norm of all gradients as if they were one vector: a float32 scalar on their device.  Sums in 64 bits."""
-    grads, dev = _check_gradients("grad_norm", grads)
-    if not grads:
-        return torch.zeros(())
-    _any_order("grad_norm", grads)
-    return _norm_and_factor(grads, math.inf, dev)[0]
+    grads = _gradients("grad_norm", grads)
+    return _norm_and_factor(grads, math.inf)[0] if len(grads) else torch.zeros(())
 
 
 @torch.no_grad()
@@ -122,22 +139,19 @@ def clip_grads_(grads, max_norm):
     """Scale all gradients in place by min(1, max_norm / (norm + 1e-6)) and return their norm before that (float32 scalar on their
     device).  Gradients within the limit are not written.  Mixed float32 / bfloat16 / float16 tensors are one vector."""
     max_norm = _limit("clip_grads_", max_norm)
-    grads, dev = _check_gradients("clip_grads_", grads)
-    if not grads:
+    grads = _gradients("clip_grads_", grads)
+    if not len(grads):
         return torch.zeros(())
-    _any_order("clip_grads_", grads)
-    out = _norm_and_factor(grads, max_norm, dev)
-    n = len(grads)
-    with torch.cuda.device(dev):
-        check(_lib.lib().dtt_grad_scale(n, _pointers(grads), _longs([g.numel() for g in grads]),
-                                        (ctypes.c_int * n)(*[_DTYPES[g.dtype] for g in grads]), ptr(out[1:]), stream_ptr(dev)), "grad_scale")
-    _written(grads)
+    out = _norm_and_factor(grads, max_norm)
+    with torch.cuda.device(out.device):
+        check(_lib.lib().dtt_grad_scale(len(grads), grads.ptrs, grads.counts, grads.types, out.data_ptr() + 4, stream_ptr(out.device)), "grad_scale")
+    _written(grads.tensors)
     return out[0]
 
 
 @torch.no_grad()
 def clip_grad_norm_(parameters, max_norm):
-    """torch.nn.utils.clip_grad_norm_ (2-norm) in three launches: clip_grads_ over the gradients of `parameters` (a tensor or an
+    """torch.nn.utils.clip_grad_norm_ (2-norm) in a few launches: clip_grads_ over the gradients of `parameters` (a tensor or an
     iterable; those without a gradient are left out, a gradient that is an expanded view is made dense first)."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     grads = []
@@ -152,96 +166,112 @@ def clip_grad_norm_(parameters, max_norm):
 
 
 # ------------------------------------------------------------------------------------------------ AdamW
-def _per_tensor(what, name, value, n):
+def _numbers(what, name, value, n):
+    """One number, or a list of n, as the array of doubles that the library takes."""
     if isinstance(value, (list, tuple)):
         if len(value) != n:
             raise ValueError("%s: %d values of %s for %d tensors" % (what, len(value), name, n))
-        return list(value)
-    return [value] * n
+        values = array("d", value)
+        if n and not min(values) >= 0.0:
+            raise ValueError("%s: %s must not be negative (got %r)" % (what, name, min(values)))
+        return values
+    if not value >= 0.0:
+        raise ValueError("%s: %s must not be negative (got %r)" % (what, name, value))
+    return array("d", [value]) * n
 
 
 class _Step:
     """The arguments of one step, checked; `launch` sends the tensors of each element type."""
 
-    def __init__(self, what, params, grads, moments, steps, lr, betas, eps, weight_decay, max_norm, skip_nonfinite, clip):
+    def __init__(self, what, params, grads, moments, types, steps, lr, betas, eps, weight_decay, max_norm, skip_nonfinite, clip):
         self.what = what
-        params, grads, steps = list(params), list(grads), list(steps)
-        moments = [list(x) for x in moments]
-        n = len(params)
-        if any(len(x) != n for x in [grads, steps] + moments):
-            raise ValueError("%s: the lists differ in length (%s)" % (what, ", ".join(str(len(x)) for x in [params, grads, steps] + moments)))
+        lists = [list(x) for x in (params, grads, steps) + tuple(moments)]
+        n = len(lists[0])
+        if any(len(x) != n for x in lists):
+            raise ValueError("%s: the lists differ in length (%s)" % (what, ", ".join(str(len(x)) for x in lists)))
         self.beta1, self.beta2 = (float(b) for b in betas)
         self.eps = float(eps)
         if not (0.0 <= self.beta1 < 1.0 and 0.0 <= self.beta2 < 1.0):
             raise ValueError("%s: betas must lie in [0, 1) (got %r)" % (what, betas))
         if not self.eps >= 0.0:
             raise ValueError("%s: eps must not be negative (got %r)" % (what, eps))
-        self.max_norm = None if max_norm is None else _limit(what, max_norm)
+        max_norm = None if max_norm is None else _limit(what, max_norm)
         self.skip_nonfinite = bool(skip_nonfinite)
         if clip is not None and (max_norm is not None or clip.dtype != torch.float32 or tuple(clip.shape) != (2,) or not clip.is_contiguous()):
             raise ValueError("%s: clip is norm and factor, two float32, and stands in place of max_norm" % what)
-        self.lr, self.lr_device = [], []
-        for x in _per_tensor(what, "lr", lr, n):
-            if isinstance(x, torch.Tensor):
+        # rates in device memory stand beside numbers of 0
+        self.rates = None
+        rates = lr if isinstance(lr, (list, tuple)) else [lr]
+        on_device = [x for x in rates if isinstance(x, torch.Tensor)]
+        if on_device:
+            for x in on_device:
                 if x.numel() != 1 or x.dtype != torch.float32:
                     raise TypeError("%s: a learning rate in device memory is one float32 (got %s, %s)" % (what, tuple(x.shape), x.dtype))
-                self.lr.append(0.0)
-                self.lr_device.append(x)
-            else:
-                if not x >= 0.0:
-                    raise ValueError("%s: lr must not be negative (got %r)" % (what, x))
-                self.lr.append(float(x))
-                self.lr_device.append(None)
-        self.decay = [float(x) for x in _per_tensor(what, "weight_decay", weight_decay, n)]
-        if not all(x >= 0.0 for x in self.decay):
-            raise ValueError("%s: weight_decay must not be negative" % what)
-        for p, g, s in zip(params, grads, steps):
-            if not all(isinstance(t, torch.Tensor) for t in (p, g, s)):
-                raise TypeError("%s: expected tensors" % what)
-            if p.dtype not in _DTYPES or p.layout != torch.strided:
-                raise TypeError("%s: parameters must be dense float32, bfloat16 or float16 tensors (got %s, %s)" % (what, p.dtype, p.layout))
-            if g.dtype != p.dtype or g.layout != torch.strided:
-                raise TypeError("%s: a gradient has its parameter's type (got %s, %s for %s)" % (what, g.dtype, g.layout, p.dtype))
-            if g.shape != p.shape:
-                raise ValueError("%s: a gradient has its parameter's shape (got %s for %s)" % (what, tuple(g.shape), tuple(p.shape)))
-            if not _dense(p):
-                raise ValueError("%s: parameters must be dense (got shape %s, strides %s)" % (what, tuple(p.shape), p.stride()))
-            if s.dtype != torch.float32 or s.numel() != 1:
-                raise TypeError("%s: a step counter is one float32 (got %s, %s)" % (what, tuple(s.shape), s.dtype))
-        self.dev = _device_of(what, params + grads + steps + [x for x in self.lr_device + [clip] if x is not None] + [t for x in moments for t in x])
-        # a gradient in another order of its dimensions (or an expanded one) is brought into the parameter's
-        grads = [g if _same_order(p, g) else torch.empty_like(p).copy_(g) for p, g in zip(params, grads)]
-        self.params, self.grads, self.moments, self.steps, self.clip = params, grads, moments, steps, clip
-        if self.clip is None and params and (self.max_norm is not None or self.skip_nonfinite):
-            self.clip = _norm_and_factor(grads, math.inf if self.max_norm is None else self.max_norm, self.dev)
-
-    def check_moments(self, dtype, lists):
-        for x in lists:
-            for p, t in zip(self.params, x):
-                if t.dtype != dtype:
-                    raise TypeError("%s: moments must be %s (got %s)" % (self.what, dtype, t.dtype))
-                if t.shape != p.shape or not _same_order(p, t):
-                    raise ValueError("%s: moments have their parameter's shape and memory order (got %s, strides %s for %s, strides %s)" %
-                                     (self.what, tuple(t.shape), t.stride(), tuple(p.shape), p.stride()))
+            rates = list(rates) if isinstance(lr, (list, tuple)) else [lr] * n
+            self.rates = array("Q", [x.data_ptr() if isinstance(x, torch.Tensor) else 0 for x in rates])
+            lr = [0.0 if isinstance(x, torch.Tensor) else x for x in rates]
+        self.lr = _numbers(what, "lr", lr, n)
+        self.decay = _numbers(what, "weight_decay", weight_decay, n)
+        self.n = n
+        if n == 0:
+            return
+        p, g, s = (_List(what, x) for x in lists[:3])
+        p.floats(what, "parameters").dense(what, "parameters")
+        if g.types != p.types:
+            raise TypeError("%s: a gradient has its parameter's type (got %s for %s)" % ((what,) + next(
+                (y.dtype if y.layout == torch.strided else y.layout, x.dtype) for x, y in zip(lists[0], lists[1])
+                if x.dtype != y.dtype or y.layout != torch.strided)))
+        at = _tensorlist().differ(lists[0], lists[1])
+        while at >= 0:
+            x, y = lists[0][at >> 1], lists[1][at >> 1]
+            if at & 1 == 0:
+                raise ValueError("%s: a gradient has its parameter's shape (got %s for %s)" % (what, tuple(y.shape), tuple(x.shape)))
+            # a gradient in another order of its dimensions (or an expanded one) is brought into the parameter's
+            lists[1] = [y if x.shape != y.shape or _same_order(x, y) else torch.empty_like(x).copy_(y) for x, y in zip(lists[0], lists[1])]
+            g = _List(what, lists[1])
+            at = _tensorlist().differ(lists[0], lists[1])
+        if s.type != 0 or s.counts != _ONE * n:
+            bad = next(t for t in lists[2] if t.dtype != torch.float32 or t.numel() != 1 or t.layout != torch.strided)
+            raise TypeError("%s: a step counter is one float32 (got %s, %s)" % (what, tuple(bad.shape), bad.dtype))
+        m = [_List(what, x) for x in lists[3:]]
+        extra = on_device + ([clip] if clip is not None else [])
+        self.dev = _device_of(what, [p, g, s] + m + ([_List(what, extra)] if extra else []))
+        for x, want in zip(m, types):
+            if x.type != want:
+                raise TypeError("%s: moments must be %s (got %s)" % (what, "float32" if want == 0 else "uint8", sorted({str(t.dtype) for t in x.tensors})))
+            at = _tensorlist().differ(lists[0], x.tensors)
+            if at >= 0:
+                t, q = x.tensors[at >> 1], lists[0][at >> 1]
+                raise ValueError("%s: moments have their parameter's shape and memory order (got %s, strides %s for %s, strides %s)" %
+                                 (what, tuple(t.shape), t.stride(), tuple(q.shape), q.stride()))
+        if clip is None and (max_norm is not None or self.skip_nonfinite):
+            clip = _norm_and_factor(g, math.inf if max_norm is None else max_norm)
+        self.params, self.grads, self.steps, self.moments, self.clip = p, g, s, m, clip
 
     def launch(self, call):
-        """call(index list, common arguments) once per element type among the parameters."""
-        by_type = {}
-        for i, p in enumerate(self.params):
-            by_type.setdefault(p.dtype, []).append(i)
+        """call(parts of one element type: lists, lr, device rates, decay, at; tail) for every element type among the parameters.
+        Returns the norm."""
+        if self.n == 0:
+            return None
+        lists = [self.params, self.grads, self.steps] + self.moments
+        groups = [(self.params.type, lists, self.lr, self.rates, self.decay, None)]
+        if self.params.type == -2:
+            groups = []
+            by_type = {}
+            for i, t in enumerate(array("i", self.params.types)):
+                by_type.setdefault(t, []).append(i)
+            for t, at in by_type.items():
+                groups.append((t, [_List(self.what, [x.tensors[i] for i in at]) for x in lists], array("d", [self.lr[i] for i in at]),
+                               None if self.rates is None else array("Q", [self.rates[i] for i in at]), array("d", [self.decay[i] for i in at]), at))
         L = _lib.lib()
-        with torch.cuda.device(self.dev):
-            for dtype, at in by_type.items():
-                n = len(at)
-                pick = (lambda x: x) if n == len(self.params) else (lambda x: [x[i] for i in at])
-                nbytes = L.dtt_adamw_workspace_bytes(n)
-                ws = torch.empty(nbytes, dtype=torch.uint8, device=self.params[at[0]].device)
-                rates = pick(self.lr_device)
-                rates = None if all(x is None for x in rates) else (ctypes.c_void_p * n)(*[None if x is None else x.data_ptr() for x in rates])
-                call(L, n, at, pick, _DTYPES[dtype], _longs([p.numel() for p in pick(self.params)]), _pointers(pick(self.steps)),
-                     (ctypes.c_double * n)(*pick(self.lr)), rates, (ctypes.c_double * n)(*pick(self.decay)),
-                     (ptr(self.clip), int(self.skip_nonfinite), ptr(ws), nbytes, stream_ptr(self.dev)))
-        _written(self.params)
+        device = self.params.tensors[0].device
+        with torch.cuda.device(device):
+            for dtype, parts, lr, rates, decay, at in groups:
+                nbytes = L.dtt_adamw_workspace_bytes(len(parts[0]))
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+                call(L, len(parts[0]), dtype, [x.ptrs for x in parts], parts[0].counts, lr.tobytes(), None if rates is None else rates.tobytes(),
+                     decay.tobytes(), at, (ptr(self.clip), int(self.skip_nonfinite), ptr(ws), nbytes, stream_ptr(device)))
+        _written(*[x.tensors for x in [self.params, self.steps] + self.moments])
         return None if self.clip is None else self.clip[0]
 
 
@@ -257,18 +287,12 @@ def adamw_(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999
     max_norm: c = min(1, max_norm / (norm + 1e-6)) of the norm over all gradients (which stay as they are), else c = 1.
     skip_nonfinite: where that norm is infinite or NaN, nothing changes, the counters neither.  clip: norm and factor computed before
     (float32, 2 entries), in place of max_norm.  Returns the norm (float32 scalar on the device), or None without any of the three."""
-    s = _Step("adamw_", params, grads, (exp_avgs, exp_avg_sqs), steps, lr, betas, eps, weight_decay, max_norm, skip_nonfinite, clip)
-    if not s.params:
-        return None
-    s.check_moments(torch.float32, s.moments)
+    s = _Step("adamw_", params, grads, (exp_avgs, exp_avg_sqs), (0, 0), steps, lr, betas, eps, weight_decay, max_norm, skip_nonfinite, clip)
 
-    def call(L, n, at, pick, dtype, numel, counters, rates, rates_device, decay, tail):
-        check(L.dtt_adamw_step(n, dtype, _pointers(pick(s.params)), _pointers(pick(s.grads)), _pointers(pick(s.moments[0])),
-                               _pointers(pick(s.moments[1])), numel, counters, rates, rates_device, decay, s.beta1, s.beta2, s.eps, *tail),
-              "adamw_")
-    norm = s.launch(call)
-    _written([t for x in s.moments for t in x] + s.steps)
-    return norm
+    def call(L, n, dtype, ptrs, numel, rates, rates_device, decay, at, tail):
+        p, g, counters, m, v = ptrs
+        check(L.dtt_adamw_step(n, dtype, p, g, m, v, numel, counters, rates, rates_device, decay, s.beta1, s.beta2, s.eps, *tail), "adamw_")
+    return s.launch(call)
 
 
 def blocks_of(numel):
@@ -285,56 +309,63 @@ def adamw8_(params, grads, exp_avgs, exp_avg_sqs, bases, steps, *, lr, betas=(0.
     2^-15.7 below its block's largest is not moved.  The rounding of a moment is dithered, right on average, by a hash of seed, ids
     (default: the position in the list), step counter and element; the same inputs give the same codes.  Infinite and NaN moments stay
     in their element, as NaN."""
-    s = _Step("adamw8_", params, grads, (exp_avgs, exp_avg_sqs, bases), steps, lr, betas, eps, weight_decay, max_norm, skip_nonfinite, clip)
-    ids = list(range(len(s.params))) if ids is None else [int(i) for i in ids]
-    if len(ids) != len(s.params):
-        raise ValueError("adamw8_: %d ids for %d tensors" % (len(ids), len(s.params)))
-    if not s.params:
+    bases = list(bases)
+    s = _Step("adamw8_", params, grads, (exp_avgs, exp_avg_sqs), (_UINT8, _UINT8), steps, lr, betas, eps, weight_decay, max_norm, skip_nonfinite,
+              clip)
+    ids = None if ids is None else [int(i) & 0xFFFFFFFF for i in ids]
+    if len(bases) != s.n or (ids is not None and len(ids) != s.n):
+        raise ValueError("adamw8_: %d bases and %s ids for %d tensors" % (len(bases), "no" if ids is None else len(ids), s.n))
+    if s.n == 0:
         return None
-    s.check_moments(torch.uint8, s.moments[:2])
-    _check_bases("adamw8_", s.params, s.moments[2])
+    _check_bases("adamw8_", s.params, _List("adamw8_", bases), s.dev)
 
-    def call(L, n, at, pick, dtype, numel, counters, rates, rates_device, decay, tail):
-        check(L.dtt_adamw8_step(n, dtype, _pointers(pick(s.params)), _pointers(pick(s.grads)), _pointers(pick(s.moments[0])),
-                                _pointers(pick(s.moments[1])), _pointers(pick(s.moments[2])), numel, counters, rates, rates_device, decay,
-                                (ctypes.c_uint * n)(*[i & 0xFFFFFFFF for i in pick(ids)]), int(seed) & 0xFFFFFFFF, s.beta1, s.beta2, s.eps,
-                                *tail), "adamw8_")
+    def call(L, n, dtype, ptrs, numel, rates, rates_device, decay, at, tail):
+        p, g, counters, m, v = ptrs
+        which, names = bases, ids
+        if at is not None:
+            which, names = [bases[i] for i in at], [at[k] if ids is None else ids[i] for k, i in enumerate(at)]
+        check(L.dtt_adamw8_step(n, dtype, p, g, m, v, _tensorlist().describe(which)[0], numel, counters, rates, rates_device, decay,
+                                None if names is None else array("I", names).tobytes(), int(seed) & 0xFFFFFFFF, s.beta1, s.beta2, s.eps, *tail),
+              "adamw8_")
     norm = s.launch(call)
-    _written([t for x in s.moments for t in x] + s.steps)
+    _written(bases)
     return norm
 
 
-def _check_bases(what, like, bases):
-    for t, b in zip(like, bases):
-        if b.dtype != torch.int16 or tuple(b.shape) != (blocks_of(t.numel()), 2) or not b.is_contiguous():
-            raise ValueError("%s: bases are int16, contiguous, two for each %d elements (got %s, %s for %d elements)" %
-                             (what, BLOCK, b.dtype, tuple(b.shape), t.numel()))
+def _check_bases(what, like, bases, dev):
+    counts = array("q", like.counts)
+    if bases.type != _INT16 or array("q", bases.counts) != array("q", [blocks_of(n) * 2 for n in counts]) or \
+            not all(b.dim() == 2 and b.shape[1] == 2 and b.is_contiguous() for b in bases.tensors):
+        raise ValueError("%s: bases are int16, contiguous, (blocks_of(numel), 2): two for each %d elements (got %s for %s elements)" %
+                         (what, BLOCK, [(str(b.dtype), tuple(b.shape)) for b in bases.tensors][:8], list(counts)[:8]))
+    if _device_of(what, [bases]) != dev:
+        raise ValueError("%s: all tensors must be on one device" % what)
 
 
 @torch.no_grad()
 def unpack_moments_(exp_avgs, exp_avg_sqs, bases, out_avgs, out_avg_sqs):
     """Write the values that 8-bit moments stand for into out_avgs / out_avg_sqs (all float32 or all bfloat16, which holds them exactly;
     in the codes' shape and memory order)."""
+    what = "unpack_moments_"
     lists = [list(x) for x in (exp_avgs, exp_avg_sqs, bases, out_avgs, out_avg_sqs)]
     n = len(lists[0])
     if any(len(x) != n for x in lists):
-        raise ValueError("unpack_moments_: the lists differ in length (%s)" % ", ".join(str(len(x)) for x in lists))
+        raise ValueError("%s: the lists differ in length (%s)" % (what, ", ".join(str(len(x)) for x in lists)))
     if n == 0:
         return
-    dev = _device_of("unpack_moments_", [t for x in lists for t in x])
-    dtype = lists[3][0].dtype
-    if dtype not in (torch.float32, torch.bfloat16) or any(t.dtype != dtype for t in lists[3] + lists[4]):
-        raise TypeError("unpack_moments_: the values come as float32 or as bfloat16")
-    for a, b, x, y in zip(lists[0], lists[1], lists[3], lists[4]):
-        if a.dtype != torch.uint8 or b.dtype != torch.uint8:
-            raise TypeError("unpack_moments_: codes are uint8 (got %s, %s)" % (a.dtype, b.dtype))
-        if not _dense(a) or not all(t.shape == a.shape and _same_order(a, t) for t in (b, x, y)):
-            raise ValueError("unpack_moments_: codes and values have one shape and memory order")
-    _check_bases("unpack_moments_", lists[0], lists[2])
+    m, v, b, x, y = (_List(what, t) for t in lists)
+    if x.type not in (0, 1) or y.type != x.type:
+        raise TypeError("%s: the values come as float32 or as bfloat16" % what)
+    if m.type != _UINT8 or v.type != _UINT8:
+        raise TypeError("%s: codes are uint8" % what)
+    m.dense(what, "codes")
+    if any(_tensorlist().differ(lists[0], t) >= 0 for t in (lists[1], lists[3], lists[4])):
+        raise ValueError("%s: codes and values have one shape and memory order" % what)
+    dev = _device_of(what, [m, v, x, y])
+    _check_bases(what, m, b, dev)
     with torch.cuda.device(dev):
-        check(_lib.lib().dtt_adamw8_unpack(n, _pointers(lists[0]), _pointers(lists[1]), _pointers(lists[2]), _longs([t.numel() for t in lists[0]]),
-                                           _DTYPES[dtype], _pointers(lists[3]), _pointers(lists[4]), stream_ptr(dev)), "unpack_moments_")
-    _written(lists[3] + lists[4])
+        check(_lib.lib().dtt_adamw8_unpack(n, m.ptrs, v.ptrs, b.ptrs, m.counts, x.type, x.ptrs, y.ptrs, stream_ptr(dev)), what)
+    _written(lists[3], lists[4])
 
 
 @torch.no_grad()
@@ -492,14 +523,15 @@ class GroupedAdamW(torch.optim.Optimizer):
                 work.setdefault((tuple(g["betas"]), g["eps"]), []).append((p, grad, g["lr"], g["weight_decay"], place))
         if not grads:
             return loss
-        _device_of("GroupedAdamW", grads)
+        _device_of("GroupedAdamW", [_List("GroupedAdamW", grads)])
         if fresh:
             self._make_state(fresh)
         clip = None
         if self.max_norm is not None or self.skip_nonfinite:
-            dense = [g if _dense(g) else g.contiguous() for g in grads]
-            checked, dev = _check_gradients("GroupedAdamW", dense)
-            clip = _norm_and_factor(checked, math.inf if self.max_norm is None else self.max_norm, dev)
+            checked = _List("GroupedAdamW", grads).floats("GroupedAdamW", "gradients")
+            if checked.odd >= 0:
+                checked = _List("GroupedAdamW", [g if _dense(g) else g.contiguous() for g in grads])
+            clip = _norm_and_factor(checked, math.inf if self.max_norm is None else self.max_norm)
             self.grad_norm = clip[0]
         for (betas, eps), rows in work.items():
             states = []
