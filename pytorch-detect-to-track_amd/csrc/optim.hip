@@ -297,20 +297,84 @@ struct Step8Table {
   const void* g[kMaxStep8];
   unsigned char* m[kMaxStep8];
   unsigned char* v[kMaxStep8];
-  short* base[kMaxStep8];   // (blocks, 2)
+  int* base[kMaxStep8];   // per block: m in the low half, v in the high one
   long numel[kMaxStep8];
   int block0[kMaxStep8];
   int n;
 };
-constexpr int kStep8Elems = kThreads * 16;   // elements per workgroup: 16 blocks
+constexpr int kWaveBlocks = 4;                                       // blocks that a wave holds at a time
+constexpr int kStep8Elems = kThreads / 64 * kWaveBlocks * kBlock;    // elements per workgroup
 
-__device__ __forceinline__ int wave_max(int x) {
-#pragma unroll
-  for (int s = 32; s > 0; s >>= 1) x = max(x, __shfl_xor(x, s));
-  return x;
+__device__ __forceinline__ unsigned max_halves(unsigned a, unsigned b) {
+  typedef unsigned short Pair __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(Pair, a), __builtin_bit_cast(Pair, b)));
+}
+// both halves' maxima over the wave, as a scalar: within 16 lanes by lane swaps, then row by row into the last lane
+template <int CTRL, int ROWS> __device__ __forceinline__ unsigned max_dpp(unsigned x) {
+  return max_halves(x, (unsigned)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ unsigned wave_max_halves(unsigned x) {
+  x = max_dpp<0xB1, 0xF>(x);    // quad_perm 1 0 3 2
+  x = max_dpp<0x4E, 0xF>(x);    // quad_perm 2 3 0 1
+  x = max_dpp<0x141, 0xF>(x);   // row_half_mirror
+  x = max_dpp<0x140, 0xF>(x);   // row_mirror
+  x = max_dpp<0x142, 0xA>(x);   // row_bcast15 into rows 1, 3
+  x = max_dpp<0x143, 0xC>(x);   // row_bcast31 into rows 2, 3
+  return (unsigned)__builtin_amdgcn_readlane((int)x, 63);
 }
 
-// A wave owns a block: four elements per lane.
+// The levels of four elements with their dither (at most 0x800), m in the low half, v in the high one.  r: the first element's hash
+// product, dr: its step to the next.
+__device__ __forceinline__ void levels4(const float (&m)[4], const float (&v)[4], unsigned r, unsigned dr, unsigned (&q)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j, r += dr) {
+    const unsigned um = ((r >> 12) & 0xFFFF0u) | 8u, uv = ((r << 4) & 0xFFFF0u) | 8u;
+    const unsigned qm = ((__float_as_uint(m[j]) & 0x7FFFFFFFu) + um) >> 20, qv = ((__float_as_uint(v[j]) & 0x7FFFFFFFu) + uv) >> 20;
+    q[j] = qm | qv << 16;
+  }
+}
+
+// Bases of the block from the wave's largest levels, and the four elements' codes.
+__device__ __forceinline__ int codes4(const float (&m)[4], const float (&v)[4], const unsigned (&q)[4], unsigned& cm, unsigned& cv) {
+  unsigned top = wave_max_halves(max_halves(max_halves(q[0], q[1]), max_halves(q[2], q[3])));
+  int flag = 0;
+  if (__builtin_expect((top & 0xFFFFu) >= (unsigned)kInfLevel || (top >> 16) >= (unsigned)kInfLevel, 0)) {   // uniform, rare
+    flag = kNanFlag;
+    unsigned t = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      t = max_halves(t, ((q[j] & 0xFFFFu) < (unsigned)kInfLevel ? q[j] & 0xFFFFu : 0u) | ((q[j] >> 16) < (unsigned)kInfLevel ? q[j] & 0xFFFF0000u : 0u));
+    top = wave_max_halves(t);
+  }
+  const int bm = max((int)(top & 0xFFFFu) - 126, 0), bv = max((int)(top >> 16) - 254, 0);
+  cm = cv = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int qm = (int)(q[j] & 0xFFFFu), qv = (int)(q[j] >> 16);
+    int lm = max(qm - bm, 0), lv = max(qv - bv, v[j] > 0.f ? 1 : 0);
+    if (flag) {
+      lm = qm >= kInfLevel ? 127 : lm;
+      lv = qv >= kInfLevel ? 255 : lv;
+    }
+    cm |= ((unsigned)lm | (m[j] < 0.f ? 128u : 0u)) << (8 * j);
+    cv |= (unsigned)lv << (8 * j);
+  }
+  return bm | bv << 16 | flag | flag << 16;
+}
+
+__device__ __forceinline__ void decode4(unsigned cm, unsigned cv, int base, float (&m)[4], float (&v)[4]) {
+  const int bm = base & 0xFFFF, bv = base >> 16;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    m[j] = decode_m((cm >> (8 * j)) & 255u, bm);
+    v[j] = decode_v((cv >> (8 * j)) & 255u, bv);
+  }
+}
+
+typedef unsigned Word __attribute__((aligned(1)));   // four codes, at any address
+
+// A wave holds four blocks: a lane has four neighbours of each, so that all of the wave's accesses are runs of memory (1 KiB of fp32
+// parameters, 256 bytes of codes), and all loads are on their way before the first is used.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void adamw8_step_kernel(Step8Table tab, const Factors* __restrict__ factors,
                                                                const float* __restrict__ clip, int skip_nonfinite, Consts k) {
@@ -322,57 +386,80 @@ __global__ __launch_bounds__(kThreads) void adamw8_step_kernel(Step8Table tab, c
   const T* g = static_cast<const T*>(tab.g[i]);
   unsigned char* cm = tab.m[i];
   unsigned char* cv = tab.v[i];
-  short* base = tab.base[i];
   const long numel = tab.numel[i];
-  const long first = (long)((int)blockIdx.x - tab.block0[i]) * kStep8Elems;
-  for (int u = 0; u < kStep8Elems / kThreads / 4; ++u) {
-    const long e0 = first + (long)u * kThreads * 4 + (threadIdx.x >> 6) * kBlock;   // the wave's block
-    if (e0 >= numel) return;
-    const long e = e0 + (threadIdx.x & 63) * 4;
-    const int bm = base[(e0 / kBlock) * 2], bv = base[(e0 / kBlock) * 2 + 1];
-    const unsigned h = mix32((unsigned)(e >> 3) ^ f.key);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const long e0 = (long)((int)blockIdx.x - tab.block0[i]) * kStep8Elems + wave * (kWaveBlocks * kBlock);
+  if (e0 >= numel) return;
+  int* base = tab.base[i] + e0 / kBlock;
+  const long e = e0 + lane * 4;
+  if (e0 + kWaveBlocks * kBlock <= numel) {
+    float xp[kWaveBlocks][4], xg[kWaveBlocks][4];
+    unsigned um[kWaveBlocks], uv[kWaveBlocks];
+    int b[kWaveBlocks];
+#pragma unroll
+    for (int u = 0; u < kWaveBlocks; ++u) {
+      um[u] = *reinterpret_cast<const Word*>(cm + e + u * kBlock);
+      uv[u] = *reinterpret_cast<const Word*>(cv + e + u * kBlock);
+      load_f32<T, 4>(g + e + u * kBlock, xg[u]);
+      load_f32<T, 4>(p + e + u * kBlock, xp[u]);
+      b[u] = base[u];
+    }
+#pragma unroll
+    for (int u = 0; u < kWaveBlocks; ++u) {
+      float xm[4], xv[4];
+      decode4(um[u], uv[u], b[u], xm, xv);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) adamw_element(xp[u][j], xg[u][j] * c, xm[j], xv[j], k, f);
+      store_f32<T, 4>(p + e + u * kBlock, xp[u]);
+      const unsigned h = mix32((unsigned)((e + u * kBlock) >> 3) ^ f.key);
+      unsigned q[4];
+      levels4(xm, xv, (lane & 1) ? h * 9u : h, 2u * h, q);
+      unsigned wm, wv;
+      b[u] = codes4(xm, xv, q, wm, wv);
+      *reinterpret_cast<Word*>(cm + e + u * kBlock) = wm;
+      *reinterpret_cast<Word*>(cv + e + u * kBlock) = wv;
+    }
+    if (lane == 0) {
+#pragma unroll
+      for (int u = 0; u < kWaveBlocks; ++u) base[u] = b[u];
+    }
+    return;
+  }
+  // the end of a tensor: elements behind it count as zeros of the block
+  for (int u = 0; u < kWaveBlocks && e0 + u * kBlock < numel; ++u) {
+    const long e1 = e + u * kBlock;
+    const int b = base[u];
     float xm[4], xv[4];
-    int qm[4], qv[4], top_m = 0, top_v = 0;
-    bool odd = false;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      xm[j] = xv[j] = 0.f; qm[j] = qv[j] = 0;
-      if (e + j < numel) {
-        xm[j] = decode_m(cm[e + j], bm);
-        xv[j] = decode_v(cv[e + j], bv);
-        float xp = (float)p[e + j];
-        adamw_element(xp, (float)g[e + j] * c, xm[j], xv[j], k, f);
-        p[e + j] = (T)xp;
-        const unsigned r = h * (2u * (unsigned)((e + j) & 7) + 1u);
-        qm[j] = (int)(((__float_as_uint(xm[j]) & 0x7FFFFFFFu) + (r >> 16) * 16u + 8u) >> 20);
-        qv[j] = (int)(((__float_as_uint(xv[j]) & 0x7FFFFFFFu) + (r & 0xFFFFu) * 16u + 8u) >> 20);
-        odd = odd || qm[j] >= kInfLevel || qv[j] >= kInfLevel;
-        if (qm[j] < kInfLevel) top_m = max(top_m, qm[j]);
-        if (qv[j] < kInfLevel) top_v = max(top_v, qv[j]);
+      xm[j] = xv[j] = 0.f;
+      if (e1 + j < numel) {
+        xm[j] = decode_m(cm[e1 + j], b & 0xFFFF);
+        xv[j] = decode_v(cv[e1 + j], b >> 16);
+        float xp = (float)p[e1 + j];
+        adamw_element(xp, (float)g[e1 + j] * c, xm[j], xv[j], k, f);
+        p[e1 + j] = (T)xp;
       }
     }
-    top_m = max(wave_max(top_m) - 126, 0);
-    top_v = max(wave_max(top_v) - 254, 0);
-    const int flag = __any(odd) ? kNanFlag : 0;
+    const unsigned h = mix32((unsigned)(e1 >> 3) ^ f.key);
+    unsigned q[4];
+    levels4(xm, xv, (lane & 1) ? h * 9u : h, 2u * h, q);
+    unsigned wm, wv;
+    const int nb = codes4(xm, xv, q, wm, wv);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (e + j < numel) {
-        const int lm = qm[j] >= kInfLevel ? 127 : max(qm[j] - top_m, 0);
-        const int lv = qv[j] >= kInfLevel ? 255 : max(qv[j] - top_v, xv[j] > 0.f ? 1 : 0);
-        cm[e + j] = (unsigned char)(lm | (xm[j] < 0.f ? 128 : 0));
-        cv[e + j] = (unsigned char)lv;
+      if (e1 + j < numel) {
+        cm[e1 + j] = (unsigned char)(wm >> (8 * j));
+        cv[e1 + j] = (unsigned char)(wv >> (8 * j));
       }
-    if ((threadIdx.x & 63) == 0) {
-      base[(e0 / kBlock) * 2] = (short)(top_m | flag);
-      base[(e0 / kBlock) * 2 + 1] = (short)(top_v | flag);
-    }
+    if (lane == 0) base[u] = nb;
   }
 }
 
 struct UnpackTable {
   const unsigned char* m[kMaxStep8];
   const unsigned char* v[kMaxStep8];
-  const short* base[kMaxStep8];
+  const int* base[kMaxStep8];
   void* out_m[kMaxStep8];
   void* out_v[kMaxStep8];
   long numel[kMaxStep8];
@@ -383,13 +470,38 @@ struct UnpackTable {
 template <typename T> __global__ __launch_bounds__(kThreads) void unpack_moments_kernel(UnpackTable tab) {
   const int i = owner(tab.block0, tab.n, blockIdx.x);
   const long numel = tab.numel[i];
-  const long first = (long)((int)blockIdx.x - tab.block0[i]) * kStep8Elems;
-  for (int u = 0; u < kStep8Elems / kThreads; ++u) {
-    const long e = first + (long)u * kThreads + threadIdx.x;
-    if (e >= numel) return;
-    static_cast<T*>(tab.out_m[i])[e] = (T)decode_m(tab.m[i][e], tab.base[i][(e / kBlock) * 2]);
-    static_cast<T*>(tab.out_v[i])[e] = (T)decode_v(tab.v[i][e], tab.base[i][(e / kBlock) * 2 + 1]);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const long e0 = (long)((int)blockIdx.x - tab.block0[i]) * kStep8Elems + wave * (kWaveBlocks * kBlock);
+  if (e0 >= numel) return;
+  const int* base = tab.base[i] + e0 / kBlock;
+  const long e = e0 + lane * 4;
+  const unsigned char* cm = tab.m[i] + e;
+  const unsigned char* cv = tab.v[i] + e;
+  T* out_m = static_cast<T*>(tab.out_m[i]) + e;
+  T* out_v = static_cast<T*>(tab.out_v[i]) + e;
+  if (e0 + kWaveBlocks * kBlock <= numel) {
+    unsigned um[kWaveBlocks], uv[kWaveBlocks];
+    int b[kWaveBlocks];
+#pragma unroll
+    for (int u = 0; u < kWaveBlocks; ++u) {
+      um[u] = *reinterpret_cast<const Word*>(cm + u * kBlock);
+      uv[u] = *reinterpret_cast<const Word*>(cv + u * kBlock);
+      b[u] = base[u];
+    }
+#pragma unroll
+    for (int u = 0; u < kWaveBlocks; ++u) {
+      float xm[4], xv[4];
+      decode4(um[u], uv[u], b[u], xm, xv);
+      store_f32<T, 4>(out_m + u * kBlock, xm);
+      store_f32<T, 4>(out_v + u * kBlock, xv);
+    }
+    return;
   }
+  for (int u = 0; u < kWaveBlocks && e0 + u * kBlock < numel; ++u)
+    for (int j = 0; j < 4 && e + u * kBlock + j < numel; ++j) {
+      out_m[u * kBlock + j] = (T)decode_m(cm[u * kBlock + j], base[u] & 0xFFFF);
+      out_v[u * kBlock + j] = (T)decode_v(cv[u * kBlock + j], base[u] >> 16);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -622,7 +734,7 @@ extern "C" int dtt_adamw8_step(int n, int dtype, void* const* params, const void
                   workspace_bytes, spans)) return 0;
   DTT_REQUIRE(n == 0 || (exp_avgs && exp_avg_sqs && bases), "adamw8: null pointer");
   for (int i = 0; i < n; ++i) {
-    DTT_REQUIRE(numel[i] == 0 || (exp_avgs[i] && exp_avg_sqs[i] && bases[i] && aligned_to(bases[i], 2)),
+    DTT_REQUIRE(numel[i] == 0 || (exp_avgs[i] && exp_avg_sqs[i] && bases[i] && aligned_to(bases[i], 4)),
                 "adamw8: tensor %d: null or unaligned moment", i);
     spans.add(exp_avgs[i], numel[i], true);
     spans.add(exp_avg_sqs[i], numel[i], true);
@@ -639,7 +751,7 @@ extern "C" int dtt_adamw8_step(int n, int dtype, void* const* params, const void
     int blocks = 0;
     for (int j = 0; j < tab.n; ++j) {
       const int i = i0 + j;
-      tab.p[j] = params[i]; tab.g[j] = grads[i]; tab.m[j] = exp_avgs[i]; tab.v[j] = exp_avg_sqs[i]; tab.base[j] = bases[i];
+      tab.p[j] = params[i]; tab.g[j] = grads[i]; tab.m[j] = exp_avgs[i]; tab.v[j] = exp_avg_sqs[i]; tab.base[j] = reinterpret_cast<int*>(bases[i]);
       tab.numel[j] = numel[i]; tab.block0[j] = blocks;
       const long nb = (numel[i] + kStep8Elems - 1) / kStep8Elems;
       blocks += (int)nb;
@@ -666,7 +778,7 @@ extern "C" int dtt_adamw8_unpack(int n, const unsigned char* const* exp_avgs, co
   DTT_REQUIRE(spans.s, "adamw8_unpack: out of host memory");
   for (int i = 0; i < n; ++i) {
     DTT_REQUIRE(numel[i] >= 0 && numel[i] <= kMaxNumel, "adamw8_unpack: tensor %d: bad element count", i);
-    DTT_REQUIRE(numel[i] == 0 || (exp_avgs[i] && exp_avg_sqs[i] && bases[i] && aligned_to(bases[i], 2) && out_avgs[i] && out_avg_sqs[i] &&
+    DTT_REQUIRE(numel[i] == 0 || (exp_avgs[i] && exp_avg_sqs[i] && bases[i] && aligned_to(bases[i], 4) && out_avgs[i] && out_avg_sqs[i] &&
                                   aligned_to(out_avgs[i], es) && aligned_to(out_avg_sqs[i], es)),
                 "adamw8_unpack: tensor %d: null or unaligned pointer", i);
     spans.add(exp_avgs[i], numel[i], false);
@@ -682,7 +794,7 @@ extern "C" int dtt_adamw8_unpack(int n, const unsigned char* const* exp_avgs, co
     int blocks = 0;
     for (int j = 0; j < tab.n; ++j) {
       const int i = i0 + j;
-      tab.m[j] = exp_avgs[i]; tab.v[j] = exp_avg_sqs[i]; tab.base[j] = bases[i]; tab.out_m[j] = out_avgs[i]; tab.out_v[j] = out_avg_sqs[i];
+      tab.m[j] = exp_avgs[i]; tab.v[j] = exp_avg_sqs[i]; tab.base[j] = reinterpret_cast<const int*>(bases[i]); tab.out_m[j] = out_avgs[i]; tab.out_v[j] = out_avg_sqs[i];
       tab.numel[j] = numel[i]; tab.block0[j] = blocks;
       const long nb = (numel[i] + kStep8Elems - 1) / kStep8Elems;
       blocks += (int)nb;
