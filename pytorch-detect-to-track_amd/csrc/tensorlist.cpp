@@ -140,6 +140,38 @@ PyObject* differ(PyObject*, PyObject* args) {
   return PyLong_FromLong(-1);
 }
 
+// rows_of(a, b, block, columns) -> -1, or the first i where b[i] is not a contiguous int16 matrix of `columns` columns and a row for
+// every `block` elements of a[i]
+PyObject* rows_of(PyObject*, PyObject* args) {
+  PyObject *a, *b;
+  long block, columns;
+  if (!PyArg_ParseTuple(args, "OOll", &a, &b, &block, &columns) || !is_list(a, "rows_of") || !is_list(b, "rows_of")) return nullptr;
+  const Py_ssize_t n = PyList_GET_SIZE(a);
+  if (PyList_GET_SIZE(b) != n || block < 1) {
+    PyErr_SetString(PyExc_ValueError, "rows_of: lists of different lengths");
+    return nullptr;
+  }
+  try {
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      PyObject *oa = PyList_GET_ITEM(a, i), *ob = PyList_GET_ITEM(b, i);
+      if (!THPVariable_Check(oa) || !THPVariable_Check(ob)) {
+        PyErr_SetString(PyExc_TypeError, "expected tensors");
+        return nullptr;
+      }
+      const at::Tensor &x = THPVariable_Unpack(oa), &y = THPVariable_Unpack(ob);
+      if (type_code(y) != kI16 || y.dim() != 2 || y.size(0) != (x.numel() + block - 1) / block || y.size(1) != columns || !y.is_contiguous())
+        return PyLong_FromSsize_t(i);
+    }
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  } catch (...) {
+    PyErr_SetString(PyExc_RuntimeError, "rows_of: unknown C++ exception");
+    return nullptr;
+  }
+  return PyLong_FromLong(-1);
+}
+
 // bump(list): the kernels wrote these tensors behind autograd's back; tell it, as torch's own in-place operations do
 PyObject* bump(PyObject*, PyObject* list) {
   if (!is_list(list, "bump")) return nullptr;
@@ -165,6 +197,7 @@ PyObject* bump(PyObject*, PyObject* list) {
 
 PyMethodDef methods[] = {{"describe", describe, METH_O, "addresses, element counts, types, device, common type, first not dense"},
                          {"differ", differ, METH_VARARGS, "first place where two lists differ in shape or memory order"},
+                         {"rows_of", rows_of, METH_VARARGS, "first matrix that has not a row for every block of its tensor"},
                          {"bump", bump, METH_O, "count a version of every tensor"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensorlist", "lists of tensors for multi-tensor calls", -1, methods, nullptr, nullptr, nullptr, nullptr};

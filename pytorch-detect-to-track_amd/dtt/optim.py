@@ -20,7 +20,7 @@ from . import _lib
 from ._lib import check, ptr, stream_ptr
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_UINT8, _INT16 = 3, 4
+_UINT8 = 3
 BLOCK = 256                      # elements, in memory order, that share a base of the 8-bit moments
 _NAN_FLAG = 0x4000
 _ONE = (1).to_bytes(8, "little")
@@ -317,14 +317,15 @@ def adamw8_(params, grads, exp_avgs, exp_avg_sqs, bases, steps, *, lr, betas=(0.
         raise ValueError("adamw8_: %d bases and %s ids for %d tensors" % (len(bases), "no" if ids is None else len(ids), s.n))
     if s.n == 0:
         return None
-    _check_bases("adamw8_", s.params, _List("adamw8_", bases), s.dev)
+    described = _List("adamw8_", bases)
+    _check_bases("adamw8_", s.params, described, s.dev)
 
     def call(L, n, dtype, ptrs, numel, rates, rates_device, decay, at, tail):
         p, g, counters, m, v = ptrs
-        which, names = bases, ids
+        where, names = described.ptrs, ids
         if at is not None:
-            which, names = [bases[i] for i in at], [at[k] if ids is None else ids[i] for k, i in enumerate(at)]
-        check(L.dtt_adamw8_step(n, dtype, p, g, m, v, _tensorlist().describe(which)[0], numel, counters, rates, rates_device, decay,
+            where, names = _List("adamw8_", [bases[i] for i in at]).ptrs, at if ids is None else [ids[i] for i in at]
+        check(L.dtt_adamw8_step(n, dtype, p, g, m, v, where, numel, counters, rates, rates_device, decay,
                                 None if names is None else array("I", names).tobytes(), int(seed) & 0xFFFFFFFF, s.beta1, s.beta2, s.eps, *tail),
               "adamw8_")
     norm = s.launch(call)
@@ -333,11 +334,11 @@ def adamw8_(params, grads, exp_avgs, exp_avg_sqs, bases, steps, *, lr, betas=(0.
 
 
 def _check_bases(what, like, bases, dev):
-    counts = array("q", like.counts)
-    if bases.type != _INT16 or array("q", bases.counts) != array("q", [blocks_of(n) * 2 for n in counts]) or \
-            not all(b.dim() == 2 and b.shape[1] == 2 and b.is_contiguous() for b in bases.tensors):
-        raise ValueError("%s: bases are int16, contiguous, (blocks_of(numel), 2): two for each %d elements (got %s for %s elements)" %
-                         (what, BLOCK, [(str(b.dtype), tuple(b.shape)) for b in bases.tensors][:8], list(counts)[:8]))
+    at = _tensorlist().rows_of(like.tensors, bases.tensors, BLOCK, 2)
+    if at >= 0:
+        b = bases.tensors[at]
+        raise ValueError("%s: bases are int16, contiguous, (blocks_of(numel), 2): two for each %d elements (got %s, %s, strides %s for %d elements)" %
+                         (what, BLOCK, b.dtype, tuple(b.shape), b.stride(), like.tensors[at].numel()))
     if _device_of(what, [bases]) != dev:
         raise ValueError("%s: all tensors must be on one device" % what)
 
