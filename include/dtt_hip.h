@@ -605,26 +605,26 @@ size_t dtt_grad_norm_workspace_bytes(int n, const long* numel);
 int dtt_grad_norm(int n, const void* const* grads, const long* numel, const int* dtypes, double max_norm, float* out,
                   void* workspace, size_t workspace_bytes, void* stream);
 int dtt_grad_scale(int n, void* const* grads, const long* numel, const int* dtypes, const float* factor, void* stream);
-/* One AdamW step (decoupled weight decay) of n tensors of one dtype.  Per tensor: t = ++*step;  g *= clip[1] (clip: the two floats
- * of dtt_grad_norm, or NULL);  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;
+/* One AdamW step (decoupled weight decay) of n tensors of one dtype.  Per tensor: t = ++*step;  g *= clip[1];  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;
  * p = p (1 - lr decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps).   Moments fp32, arithmetic fp32, factors of
- * t in 64 bits; p rounded once to its dtype.  lr_device: NULL, or per tensor NULL / a device float that replaces lr[i] (read when the
+ * t in 64 bits; p rounded once to its dtype.  max_norm >= 0: the call computes norm and factor of its gradients as dtt_grad_norm
+ * does, into clip (2 device floats); max_norm < 0: clip holds them already, or is NULL (no clipping).  lr_device: NULL, or per tensor NULL / a device float that replaces lr[i] (read when the
  * kernel runs).  skip_nonfinite: a norm clip[0] that is not finite leaves parameters, moments and counters as they were.
- * workspace: dtt_adamw_workspace_bytes(n), 16-byte aligned. */
-size_t dtt_adamw_workspace_bytes(int n);
+ * workspace: dtt_adamw_workspace_bytes(n, numel), 16-byte aligned. */
+size_t dtt_adamw_workspace_bytes(int n, const long* numel);
 int dtt_adamw_step(int n, int dtype, void* const* params, const void* const* grads, float* const* exp_avgs, float* const* exp_avg_sqs,
                    const long* numel, float* const* steps, const double* lr, const float* const* lr_device,
-                   const double* weight_decay, double beta1, double beta2, double eps, const float* clip, int skip_nonfinite,
-                   void* workspace, size_t workspace_bytes, void* stream);
-/* The same step with the moments in 8 bits: codes of numel bytes each, and bases, two int16 (m, v) per 256 elements in memory order
- * (all zero = moments of zero).  A code counts levels of a fixed grid -- eight per power of two, the upper 12 bits of the fp32 --
+                   const double* weight_decay, double beta1, double beta2, double eps, double max_norm, float* clip,
+                   int skip_nonfinite, void* workspace, size_t workspace_bytes, void* stream);
+/* The same step with the moments in 8 bits: codes of numel bytes each, and bases, two int16 (m, v; 4-byte aligned) per 256 elements in memory
+ * order (all zero = moments of zero).  A code counts levels of a fixed grid -- eight per power of two, the upper 12 bits of the fp32 --
  * from its block's base: m sign + 7 bits, v 8 bits; bit 14 of a base: the block holds infinities / NaN, whose code is 127 / 255.
  * Rounding is dithered (right on average: to the nearest of levels 12.5 % apart, beta2 = 0.999 would never move v) by a hash of seed,
  * ids[i] (NULL = i), step counter and element: the same inputs give the same codes. */
 int dtt_adamw8_step(int n, int dtype, void* const* params, const void* const* grads, unsigned char* const* exp_avgs,
                     unsigned char* const* exp_avg_sqs, short* const* bases, const long* numel, float* const* steps,
                     const double* lr, const float* const* lr_device, const double* weight_decay, const unsigned* ids, unsigned seed,
-                    double beta1, double beta2, double eps, const float* clip, int skip_nonfinite, void* workspace,
+                    double beta1, double beta2, double eps, double max_norm, float* clip, int skip_nonfinite, void* workspace,
                     size_t workspace_bytes, void* stream);
 /* The values that 8-bit moments stand for, as fp32 (out_dtype 0) or bf16 (1; exact: a value has four significant bits). */
 int dtt_adamw8_unpack(int n, const unsigned char* const* exp_avgs, const unsigned char* const* exp_avg_sqs, const short* const* bases,

@@ -18,8 +18,9 @@ constexpr int kThreads = 256;
 constexpr int kMaxNorm = 160;     // tensors per launch: 8 + 8 + 4 + 4 bytes each
 constexpr int kMaxStep = 80;      // 5 * 8 + 4 bytes each
 constexpr int kMaxStep8 = 72;     // 6 * 8 + 4
-constexpr int kMaxPrepare = 96;   // 4 * 8 + 4
-constexpr int kNormWorkgroups = 4096;
+constexpr int kMaxPrepare = 280;  // 8 + 4 + 1, and kMaxRates different rates
+constexpr int kMaxRates = 8;
+constexpr int kNormWorkgroups = 2048;   // 8 on a CU: all resident at once
 constexpr long kMaxNumel = 1L << 34;   // element / 8 fits the 32-bit hash input; a launch's workgroups (kMaxNumel / 4096 * kMax*) fit an int
 
 enum { kF32 = 0, kBf16 = 1, kF16 = 2 };
@@ -70,11 +71,21 @@ struct NormTable {
 };
 
 template <typename T, int N> __device__ __forceinline__ double square_sum(const T* g, long e0, long e1) {
+  constexpr int kFly = 4;   // vectors on their way per thread
   double acc[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) acc[i] = 0.0;
   long e = e0 + (long)threadIdx.x * N;
-  for (; e + N <= e1; e += (long)kThreads * N) {
+  for (; e + (kFly - 1) * kThreads * N + N <= e1; e += kFly * kThreads * N) {
+    float x[kFly][N];
+#pragma unroll
+    for (int u = 0; u < kFly; ++u) load_f32<T, N>(g + e + u * kThreads * N, x[u]);
+#pragma unroll
+    for (int u = 0; u < kFly; ++u)
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[i] = __builtin_fma((double)x[u][i], (double)x[u][i], acc[i]);
+  }
+  for (; e + N <= e1; e += kThreads * N) {
     float x[N];
     load_f32<T, N>(g + e, x);
 #pragma unroll
@@ -115,18 +126,23 @@ __global__ __launch_bounds__(kThreads) void grad_norm_kernel(NormTable tab, doub
   if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
 
-__global__ __launch_bounds__(1024) void grad_norm_finish_kernel(const double* __restrict__ partial, int n, double max_norm,
-                                                                float* __restrict__ out) {
+// The partial sums of all workgroups, in index order within a thread, then over the threads: norm and factor, in every thread.
+constexpr int kFinish = 512;   // threads
+__device__ __forceinline__ float2 finish_norm(const double* __restrict__ partial, int n, double max_norm) {
   double s = 0.0;
-  for (int i = threadIdx.x; i < n; i += 1024) s += partial[i];
-  s = workgroup_sum<16>(s);
-  if (threadIdx.x == 0) {
-    const double norm = sqrt(s);
-    // (an infinite limit asks for the norm alone; a norm that is not a number stays one in the factor, an infinite one gives 0)
-    const double f = max_norm / (norm + 1e-6);
-    out[0] = (float)norm;
-    out[1] = isinf(max_norm) ? 1.f : f < 1.0 || f != f ? (float)f : 1.f;
-  }
+#pragma unroll 4
+  for (int i = threadIdx.x; i < n; i += kFinish) s += partial[i];
+  s = workgroup_sum<kFinish / 64>(s);
+  const double norm = sqrt(s);
+  // (an infinite limit asks for the norm alone; a norm that is not a number stays one in the factor, an infinite one gives 0)
+  const double f = max_norm / (norm + 1e-6);
+  return make_float2((float)norm, isinf(max_norm) ? 1.f : f < 1.0 || f != f ? (float)f : 1.f);
+}
+
+__global__ __launch_bounds__(kFinish) void grad_norm_finish_kernel(const double* __restrict__ partial, int n, double max_norm,
+                                                                   float* __restrict__ out) {
+  const float2 r = finish_norm(partial, n, max_norm);
+  if (threadIdx.x == 0) { out[0] = r.x; out[1] = r.y; }
 }
 
 // ------------------------------------------------------------------------------------------------ scaling
@@ -165,16 +181,26 @@ __global__ __launch_bounds__(kThreads) void grad_scale_kernel(ScaleTable tab, co
 // ------------------------------------------------------------------------------------------------ what a step needs per tensor
 // One thread per tensor: t <- t + 1 in the tensor's step counter, and the step's factors in 64 bits, rounded once:
 // keep = 1 - lr * decay, size = lr / (1 - beta1^t), root = 1 / sqrt(1 - beta2^t); for 8-bit moments the key of its rounding terms.
+// Where the call clips, the same workgroup joins the norm's partial sums first (one launch less than a kernel of its own).
 // The counters live on the device, so a captured step counts on with every replay.
+struct Rate {
+  double lr;
+  const float* lr_device;   // learning rate in device memory (a schedule under a captured graph), or NULL
+  double decay;
+};
 struct PrepareTable {
   float* step[kMaxPrepare];
-  double lr[kMaxPrepare];
-  const float* lr_device[kMaxPrepare];   // learning rate in device memory (a schedule under a captured graph), or NULL
-  double decay[kMaxPrepare];
+  Rate rate[kMaxRates];
   unsigned id[kMaxPrepare];
-  double beta1, beta2;
-  unsigned seed;
+  unsigned char which[kMaxPrepare];   // entry of rate
   int n;
+  unsigned seed;
+  double beta1, beta2;
+};
+struct NormPart {
+  const double* partial;   // NULL: the call does not compute a norm, clip (or NULL) is given
+  int n;
+  double max_norm;
 };
 struct Factors {
   float keep, size, root;
@@ -191,15 +217,24 @@ __device__ __forceinline__ bool skipped(const float* clip, int skip_nonfinite) {
   return skip_nonfinite && !isfinite(clip[0]);
 }
 
-__global__ __launch_bounds__(kMaxPrepare) void adamw_prepare_kernel(PrepareTable tab, const float* __restrict__ clip,
-                                                                    int skip_nonfinite, Factors* __restrict__ factors) {
+__global__ __launch_bounds__(kFinish) void adamw_prepare_kernel(PrepareTable tab, NormPart part, float* __restrict__ clip, int skip_nonfinite,
+                                                                Factors* __restrict__ factors) {
+  bool skip = false;
+  if (part.partial) {
+    const float2 r = finish_norm(part.partial, part.n, part.max_norm);
+    if (threadIdx.x == 0) { clip[0] = r.x; clip[1] = r.y; }
+    skip = skip_nonfinite && !isfinite(r.x);
+  } else if (clip) {
+    skip = skipped(clip, skip_nonfinite);
+  }
   const int i = threadIdx.x;
-  if (i >= tab.n || (clip && skipped(clip, skip_nonfinite))) return;
+  if (i >= tab.n || skip) return;
+  const Rate rate = tab.rate[tab.which[i]];
   const float t = *tab.step[i] + 1.f;   // (exact up to 2^24 steps)
   *tab.step[i] = t;
-  const double lr = tab.lr_device[i] ? (double)*tab.lr_device[i] : tab.lr[i];
+  const double lr = rate.lr_device ? (double)*rate.lr_device : rate.lr;
   Factors f;
-  f.keep = (float)(1.0 - lr * tab.decay[i]);
+  f.keep = (float)(1.0 - lr * rate.decay);
   f.size = (float)(lr / (1.0 - pow(tab.beta1, (double)t)));
   f.root = (float)(1.0 / sqrt(1.0 - pow(tab.beta2, (double)t)));
   f.key = mix32(mix32(tab.seed + 0x9E3779B9u * (tab.id[i] + 1u)) + (unsigned)t);
@@ -511,25 +546,49 @@ int type_bytes(int dtype) { return dtype == kF32 ? 4 : 2; }
 // view of another, a shared step counter): the workgroups run in no order.
 struct Spans {
   struct Span {
-    uintptr_t lo, hi;
-    bool written;
-    bool operator<(const Span& o) const { return lo < o.lo; }
+    uintptr_t lo, hi;   // twice the addresses; hi's lowest bit says "written"
   };
   Span* s = nullptr;
-  long n = 0;
-  explicit Spans(long most) { s = static_cast<Span*>(malloc((size_t)(most > 0 ? most : 1) * sizeof(Span))); }
+  long n = 0, most;
+  explicit Spans(long most_) : most(most_ > 0 ? most_ : 1) { s = static_cast<Span*>(malloc(2 * (size_t)most * sizeof(Span))); }
   ~Spans() { free(s); }
   Spans(const Spans&) = delete;
   void add(const void* p, long bytes, bool written) {
-    if (bytes > 0) { s[n].lo = reinterpret_cast<uintptr_t>(p); s[n].hi = s[n].lo + (uintptr_t)bytes; s[n].written = written; ++n; }
+    if (bytes <= 0) return;
+    s[n].lo = reinterpret_cast<uintptr_t>(p) * 2;
+    s[n].hi = (reinterpret_cast<uintptr_t>(p) + (uintptr_t)bytes) * 2 + (written ? 1 : 0);
+    ++n;
   }
+  // Merges ascending runs: the buffers of one list mostly ascend, so that three passes do for the five lists of a step
+  // (1505 spans of 301 tensors: 12 us, where a sort takes 50).
+  void order() {
+    Span *from = s, *to = s + most;
+    for (;;) {
+      long at = 0, runs = 0;
+      while (at < n) {
+        long mid = at + 1;
+        while (mid < n && from[mid - 1].lo <= from[mid].lo) ++mid;
+        long end = mid;
+        if (mid < n) for (end = mid + 1; end < n && from[end - 1].lo <= from[end].lo;) ++end;
+        std::merge(from + at, from + mid, from + mid, from + end, to + at, [](const Span& a, const Span& b) { return a.lo < b.lo; });
+        at = end;
+        ++runs;
+      }
+      Span* t = from; from = to; to = t;
+      if (runs <= 1) break;
+    }
+    s_ordered = from;
+  }
+  const Span* s_ordered = nullptr;
   bool clash() {
-    std::sort(s, s + n);
+    order();
     uintptr_t any = 0, written = 0;
     for (long i = 0; i < n; ++i) {
-      if (s[i].lo < written || (s[i].written && s[i].lo < any)) return true;
-      if (s[i].hi > any) any = s[i].hi;
-      if (s[i].written && s[i].hi > written) written = s[i].hi;
+      const uintptr_t lo = s_ordered[i].lo, hi = s_ordered[i].hi & ~(uintptr_t)1;
+      const bool w = s_ordered[i].hi & 1;
+      if (lo < written || (w && lo < any)) return true;
+      if (hi > any) any = hi;
+      if (w && hi > written) written = hi;
     }
     return false;
   }
@@ -565,16 +624,11 @@ extern "C" size_t dtt_grad_norm_workspace_bytes(int n, const long* numel) {
   return (size_t)(blocks > 0 ? blocks : 1) * sizeof(double);
 }
 
-extern "C" int dtt_grad_norm(int n, const void* const* grads, const long* numel, const int* dtypes, double max_norm, float* out,
-                             void* workspace, size_t workspace_bytes, void* stream_) {
-  hipStream_t stream = static_cast<hipStream_t>(stream_);
-  if (!check_grads("grad_norm", n, grads, numel, dtypes)) return 0;
-  DTT_REQUIRE(out && workspace && aligned_to(workspace, 8), "grad_norm: null or unaligned pointer");
-  DTT_REQUIRE(max_norm >= 0.0, "grad_norm: max_norm must not be negative");
-  DTT_REQUIRE(workspace_bytes >= dtt_grad_norm_workspace_bytes(n, numel), "grad_norm: workspace too small");
-  double* partial = static_cast<double*>(workspace);
+namespace {
+
+// the partial sums of all tensors; returns their number, -1 after a failed launch.  dtypes: one per tensor, or NULL (all `dtype`)
+int norm_partials(int n, const void* const* grads, const long* numel, const int* dtypes, int dtype, double* partial, hipStream_t stream) {
   const long chunk = n > 0 ? norm_chunk(n, numel) : 1;
-  dtt_prof_begin("grad_norm", stream);
   int blocks = 0;
   NormTable tab;
   for (int i = 0; i < n;) {
@@ -583,15 +637,35 @@ extern "C" int dtt_grad_norm(int n, const void* const* grads, const long* numel,
     for (; i < n && tab.n < kMaxNorm; ++i) {
       if (numel[i] == 0) continue;
       const int j = tab.n++;
-      tab.g[j] = grads[i]; tab.numel[j] = numel[i]; tab.dtype[j] = dtypes[i]; tab.block0[j] = here;
+      tab.g[j] = grads[i]; tab.numel[j] = numel[i]; tab.dtype[j] = dtypes ? dtypes[i] : dtype; tab.block0[j] = here;
       here += (int)((numel[i] + chunk - 1) / chunk);
     }
     if (here == 0) break;
     hipLaunchKernelGGL(grad_norm_kernel, dim3((unsigned)here), dim3(kThreads), 0, stream, tab, partial + blocks);
-    DTT_CHECK_LAUNCH("grad_norm_kernel");
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) {
+      dtt_set_error("grad_norm_kernel: launch failed: %s", hipGetErrorString(e));
+      return -1;
+    }
     blocks += here;
   }
-  hipLaunchKernelGGL(grad_norm_finish_kernel, dim3(1), dim3(1024), 0, stream, partial, blocks, max_norm, out);
+  return blocks;
+}
+
+}  // namespace
+
+extern "C" int dtt_grad_norm(int n, const void* const* grads, const long* numel, const int* dtypes, double max_norm, float* out,
+                             void* workspace, size_t workspace_bytes, void* stream_) {
+  hipStream_t stream = static_cast<hipStream_t>(stream_);
+  if (!check_grads("grad_norm", n, grads, numel, dtypes)) return 0;
+  DTT_REQUIRE(out && workspace && aligned_to(workspace, 8), "grad_norm: null or unaligned pointer");
+  DTT_REQUIRE(max_norm >= 0.0, "grad_norm: max_norm must not be negative");
+  DTT_REQUIRE(workspace_bytes >= dtt_grad_norm_workspace_bytes(n, numel), "grad_norm: workspace too small");
+  double* partial = static_cast<double*>(workspace);
+  dtt_prof_begin("grad_norm", stream);
+  const int blocks = norm_partials(n, grads, numel, dtypes, 0, partial, stream);
+  if (blocks < 0) return 0;
+  hipLaunchKernelGGL(grad_norm_finish_kernel, dim3(1), dim3(kFinish), 0, stream, partial, blocks, max_norm, out);
   DTT_CHECK_LAUNCH("grad_norm_finish_kernel");
   dtt_prof_end("grad_norm", stream);
   return 1;
@@ -625,20 +699,22 @@ extern "C" int dtt_grad_scale(int n, void* const* grads, const long* numel, cons
   return 1;
 }
 
-extern "C" size_t dtt_adamw_workspace_bytes(int n) { return (size_t)(n > 0 ? n : 1) * sizeof(Factors); }
+extern "C" size_t dtt_adamw_workspace_bytes(int n, const long* numel) {
+  return (size_t)(n > 0 ? n : 1) * sizeof(Factors) + dtt_grad_norm_workspace_bytes(n, numel);
+}
 
 namespace {
 
 // what both steps check of their arguments; the buffers' spans are collected for the overlap check
 int check_step(const char* what, int n, int dtype, void* const* params, const void* const* grads, const long* numel, float* const* steps,
-               const double* lr, const double* decay, double beta1, double beta2, double eps, const float* clip, int skip_nonfinite,
-               const void* workspace, size_t workspace_bytes, Spans& spans) {
+               const double* lr, const double* decay, double beta1, double beta2, double eps, double max_norm, const float* clip,
+               int skip_nonfinite, const void* workspace, size_t workspace_bytes, Spans& spans) {
   DTT_REQUIRE(n >= 0 && (n == 0 || (params && grads && numel && steps && lr && decay)), "%s: null pointer", what);
   DTT_REQUIRE(dtype >= kF32 && dtype <= kF16, "%s: unknown element type %d", what, dtype);
   DTT_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "%s: betas must lie in [0, 1)", what);
   DTT_REQUIRE(eps >= 0.0, "%s: eps must not be negative", what);
-  DTT_REQUIRE(!skip_nonfinite || clip, "%s: skip_nonfinite needs the gradients' norm", what);
-  DTT_REQUIRE(workspace && aligned_to(workspace, 16) && workspace_bytes >= dtt_adamw_workspace_bytes(n), "%s: workspace too small or unaligned", what);
+  DTT_REQUIRE(max_norm == max_norm, "%s: max_norm is not a number", what);
+  DTT_REQUIRE(clip || (!skip_nonfinite && max_norm < 0.0), "%s: clipping and skip_nonfinite need a place for norm and factor", what);
   DTT_REQUIRE(spans.s, "%s: out of host memory", what);
   const int es = type_bytes(dtype);
   for (int i = 0; i < n; ++i) {
@@ -647,25 +723,44 @@ int check_step(const char* what, int n, int dtype, void* const* params, const vo
     DTT_REQUIRE(lr[i] >= 0.0 && decay[i] >= 0.0, "%s: tensor %d: learning rate and weight decay must not be negative", what, i);
     DTT_REQUIRE(numel[i] == 0 || (params[i] && grads[i] && aligned_to(params[i], es) && aligned_to(grads[i], es)),
                 "%s: tensor %d: null or unaligned pointer", what, i);
-    spans.add(params[i], numel[i] * es, true);
-    spans.add(grads[i], numel[i] * es, false);
-    spans.add(steps[i], 4, true);
   }
+  DTT_REQUIRE(workspace && aligned_to(workspace, 16) && workspace_bytes >= dtt_adamw_workspace_bytes(n, numel), "%s: workspace too small or unaligned", what);
+  for (int i = 0; i < n; ++i) spans.add(params[i], numel[i] * es, true);
+  for (int i = 0; i < n; ++i) spans.add(grads[i], numel[i] * es, false);
+  for (int i = 0; i < n; ++i) spans.add(steps[i], 4, true);
   return 1;
 }
 
-int prepare(int n, float* const* steps, const double* lr, const float* const* lr_device, const double* decay, const unsigned* ids,
-            unsigned seed, double beta1, double beta2, const float* clip, int skip_nonfinite, Factors* factors, hipStream_t stream) {
+// the norm where the call clips, then counters and factors
+int prepare(int n, int dtype, const void* const* grads, const long* numel, float* const* steps, const double* lr, const float* const* lr_device,
+            const double* decay, const unsigned* ids, unsigned seed, double beta1, double beta2, double max_norm, float* clip, int skip_nonfinite,
+            Factors* factors, hipStream_t stream) {
+  NormPart part = {nullptr, 0, 0.0};
+  if (max_norm >= 0.0) {
+    double* partial = reinterpret_cast<double*>(factors + (n > 0 ? n : 1));
+    part.n = norm_partials(n, grads, numel, nullptr, dtype, partial, stream);
+    if (part.n < 0) return 0;
+    part.partial = partial;
+    part.max_norm = max_norm;
+  }
   PrepareTable tab;
   tab.beta1 = beta1; tab.beta2 = beta2; tab.seed = seed;
-  for (int i0 = 0; i0 < n; i0 += kMaxPrepare) {
-    tab.n = n - i0 < kMaxPrepare ? n - i0 : kMaxPrepare;
-    for (int j = 0; j < tab.n; ++j) {
-      tab.step[j] = steps[i0 + j]; tab.lr[j] = lr[i0 + j]; tab.decay[j] = decay[i0 + j];
-      tab.lr_device[j] = lr_device ? lr_device[i0 + j] : nullptr;
-      tab.id[j] = ids ? ids[i0 + j] : (unsigned)(i0 + j);
+  for (int i = 0; i < n;) {
+    const int i0 = i;
+    int rates = 0;
+    for (tab.n = 0; i < n && tab.n < kMaxPrepare; ++i) {
+      const float* dev = lr_device ? lr_device[i] : nullptr;
+      int r = 0;
+      while (r < rates && !(tab.rate[r].lr == lr[i] && tab.rate[r].lr_device == dev && tab.rate[r].decay == decay[i])) ++r;
+      if (r == rates) {
+        if (rates == kMaxRates) break;   // more rates than the table holds: another launch
+        tab.rate[rates].lr = lr[i]; tab.rate[rates].lr_device = dev; tab.rate[rates].decay = decay[i];
+        ++rates;
+      }
+      const int j = tab.n++;
+      tab.step[j] = steps[i]; tab.which[j] = (unsigned char)r; tab.id[j] = ids ? ids[i] : (unsigned)i;
     }
-    hipLaunchKernelGGL(adamw_prepare_kernel, dim3(1), dim3(kMaxPrepare), 0, stream, tab, clip, skip_nonfinite, factors + i0);
+    hipLaunchKernelGGL(adamw_prepare_kernel, dim3(1), dim3(kFinish), 0, stream, tab, part, clip, skip_nonfinite, factors + i0);
     DTT_CHECK_LAUNCH("adamw_prepare_kernel");
   }
   return 1;
@@ -684,23 +779,24 @@ Consts consts(double beta1, double beta2, double eps) {
 extern "C" int dtt_adamw_step(int n, int dtype, void* const* params, const void* const* grads, float* const* exp_avgs,
                               float* const* exp_avg_sqs, const long* numel, float* const* steps, const double* lr,
                               const float* const* lr_device, const double* weight_decay, double beta1, double beta2, double eps,
-                              const float* clip, int skip_nonfinite, void* workspace, size_t workspace_bytes, void* stream_) {
+                              double max_norm, float* clip, int skip_nonfinite, void* workspace, size_t workspace_bytes, void* stream_) {
   hipStream_t stream = static_cast<hipStream_t>(stream_);
   Spans spans(5L * (n > 0 ? n : 0));
-  if (!check_step("adamw", n, dtype, params, grads, numel, steps, lr, weight_decay, beta1, beta2, eps, clip, skip_nonfinite, workspace,
+  if (!check_step("adamw", n, dtype, params, grads, numel, steps, lr, weight_decay, beta1, beta2, eps, max_norm, clip, skip_nonfinite, workspace,
                   workspace_bytes, spans)) return 0;
   DTT_REQUIRE(n == 0 || (exp_avgs && exp_avg_sqs), "adamw: null pointer");
   for (int i = 0; i < n; ++i) {
     DTT_REQUIRE(numel[i] == 0 || (exp_avgs[i] && exp_avg_sqs[i] && aligned_to(exp_avgs[i], 4) && aligned_to(exp_avg_sqs[i], 4)),
                 "adamw: tensor %d: null or unaligned moment", i);
-    spans.add(exp_avgs[i], numel[i] * 4, true);
-    spans.add(exp_avg_sqs[i], numel[i] * 4, true);
   }
+  for (int i = 0; i < n; ++i) spans.add(exp_avgs[i], numel[i] * 4, true);
+  for (int i = 0; i < n; ++i) spans.add(exp_avg_sqs[i], numel[i] * 4, true);
   DTT_REQUIRE(!spans.clash(), "adamw: two of the tensors share memory");
   Factors* factors = static_cast<Factors*>(workspace);
   const Consts k = consts(beta1, beta2, eps);
   dtt_prof_begin("adamw", stream);
-  if (!prepare(n, steps, lr, lr_device, weight_decay, nullptr, 0u, beta1, beta2, clip, skip_nonfinite, factors, stream)) return 0;
+  if (!prepare(n, dtype, grads, numel, steps, lr, lr_device, weight_decay, nullptr, 0u, beta1, beta2, max_norm, clip, skip_nonfinite, factors,
+               stream)) return 0;
   StepTable tab;
   for (int i0 = 0; i0 < n; i0 += kMaxStep) {
     tab.n = n - i0 < kMaxStep ? n - i0 : kMaxStep;
@@ -726,25 +822,26 @@ extern "C" int dtt_adamw_step(int n, int dtype, void* const* params, const void*
 extern "C" int dtt_adamw8_step(int n, int dtype, void* const* params, const void* const* grads, unsigned char* const* exp_avgs,
                                unsigned char* const* exp_avg_sqs, short* const* bases, const long* numel, float* const* steps,
                                const double* lr, const float* const* lr_device, const double* weight_decay, const unsigned* ids,
-                               unsigned seed, double beta1, double beta2, double eps, const float* clip, int skip_nonfinite,
+                               unsigned seed, double beta1, double beta2, double eps, double max_norm, float* clip, int skip_nonfinite,
                                void* workspace, size_t workspace_bytes, void* stream_) {
   hipStream_t stream = static_cast<hipStream_t>(stream_);
   Spans spans(6L * (n > 0 ? n : 0));
-  if (!check_step("adamw8", n, dtype, params, grads, numel, steps, lr, weight_decay, beta1, beta2, eps, clip, skip_nonfinite, workspace,
+  if (!check_step("adamw8", n, dtype, params, grads, numel, steps, lr, weight_decay, beta1, beta2, eps, max_norm, clip, skip_nonfinite, workspace,
                   workspace_bytes, spans)) return 0;
   DTT_REQUIRE(n == 0 || (exp_avgs && exp_avg_sqs && bases), "adamw8: null pointer");
   for (int i = 0; i < n; ++i) {
     DTT_REQUIRE(numel[i] == 0 || (exp_avgs[i] && exp_avg_sqs[i] && bases[i] && aligned_to(bases[i], 4)),
                 "adamw8: tensor %d: null or unaligned moment", i);
-    spans.add(exp_avgs[i], numel[i], true);
-    spans.add(exp_avg_sqs[i], numel[i], true);
-    spans.add(bases[i], (numel[i] + kBlock - 1) / kBlock * 4, true);
   }
+  for (int i = 0; i < n; ++i) spans.add(exp_avgs[i], numel[i], true);
+  for (int i = 0; i < n; ++i) spans.add(exp_avg_sqs[i], numel[i], true);
+  for (int i = 0; i < n; ++i) spans.add(bases[i], (numel[i] + kBlock - 1) / kBlock * 4, true);
   DTT_REQUIRE(!spans.clash(), "adamw8: two of the tensors share memory");
   Factors* factors = static_cast<Factors*>(workspace);
   const Consts k = consts(beta1, beta2, eps);
   dtt_prof_begin("adamw8", stream);
-  if (!prepare(n, steps, lr, lr_device, weight_decay, ids, seed, beta1, beta2, clip, skip_nonfinite, factors, stream)) return 0;
+  if (!prepare(n, dtype, grads, numel, steps, lr, lr_device, weight_decay, ids, seed, beta1, beta2, max_norm, clip, skip_nonfinite, factors,
+               stream)) return 0;
   Step8Table tab;
   for (int i0 = 0; i0 < n; i0 += kMaxStep8) {
     tab.n = n - i0 < kMaxStep8 ? n - i0 : kMaxStep8;
@@ -781,12 +878,12 @@ extern "C" int dtt_adamw8_unpack(int n, const unsigned char* const* exp_avgs, co
     DTT_REQUIRE(numel[i] == 0 || (exp_avgs[i] && exp_avg_sqs[i] && bases[i] && aligned_to(bases[i], 4) && out_avgs[i] && out_avg_sqs[i] &&
                                   aligned_to(out_avgs[i], es) && aligned_to(out_avg_sqs[i], es)),
                 "adamw8_unpack: tensor %d: null or unaligned pointer", i);
-    spans.add(exp_avgs[i], numel[i], false);
-    spans.add(exp_avg_sqs[i], numel[i], false);
-    spans.add(bases[i], (numel[i] + kBlock - 1) / kBlock * 4, false);
-    spans.add(out_avgs[i], numel[i] * es, true);
-    spans.add(out_avg_sqs[i], numel[i] * es, true);
   }
+  for (int i = 0; i < n; ++i) spans.add(exp_avgs[i], numel[i], false);
+  for (int i = 0; i < n; ++i) spans.add(exp_avg_sqs[i], numel[i], false);
+  for (int i = 0; i < n; ++i) spans.add(bases[i], (numel[i] + kBlock - 1) / kBlock * 4, false);
+  for (int i = 0; i < n; ++i) spans.add(out_avgs[i], numel[i] * es, true);
+  for (int i = 0; i < n; ++i) spans.add(out_avg_sqs[i], numel[i] * es, true);
   DTT_REQUIRE(!spans.clash(), "adamw8_unpack: two of the tensors share memory");
   UnpackTable tab;
   for (int i0 = 0; i0 < n; i0 += kMaxStep8) {

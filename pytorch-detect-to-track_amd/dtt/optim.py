@@ -11,13 +11,14 @@ Nothing here waits for the GPU: norms, step counters and the decision to skip a 
 captured into a graph and counts on with every replay.  A captured call keeps the addresses of the tensors it was given and a
 learning rate given as a number; a schedule under a graph passes the rate as a float32 tensor and writes to it.
 """
+import contextlib
 import math
 from array import array
 
 import torch
 
 from . import _lib
-from ._lib import check, ptr, stream_ptr
+from ._lib import check
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _UINT8 = 3
@@ -106,6 +107,18 @@ def _written(*lists):
         _tensorlist().bump(x)
 
 
+_HERE = contextlib.nullcontext()
+
+
+def _on(dev):
+    """The device of a call's tensors as the current one (a step of a few small tensors takes 20 us: no guard where none is needed)."""
+    return _HERE if torch.cuda.current_device() == dev else torch.cuda.device(dev)
+
+
+def _stream(dev):
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
 # ------------------------------------------------------------------------------------------------ gradient norm
 def _norm_and_factor(grads, max_norm):
     """(2,) float32: the norm of all gradients (a _List on one GPU) and the factor min(1, max_norm / (norm + 1e-6))."""
@@ -113,10 +126,11 @@ def _norm_and_factor(grads, max_norm):
     device = grads.tensors[0].device
     out = torch.empty(2, dtype=torch.float32, device=device)
     L = _lib.lib()
-    with torch.cuda.device(device):
-        nbytes = L.dtt_grad_norm_workspace_bytes(n, grads.counts)
-        ws = torch.empty(nbytes // 8, dtype=torch.float64, device=device)
-        check(L.dtt_grad_norm(n, grads.ptrs, grads.counts, grads.types, max_norm, ptr(out), ptr(ws), nbytes, stream_ptr(device)), "grad_norm")
+    nbytes = L.dtt_grad_norm_workspace_bytes(n, grads.counts)
+    ws = torch.empty(nbytes // 8, dtype=torch.float64, device=device)
+    with _on(grads.device):
+        check(L.dtt_grad_norm(n, grads.ptrs, grads.counts, grads.types, max_norm, out.data_ptr(), ws.data_ptr(), nbytes, _stream(grads.device)),
+              "grad_norm")
     return out
 
 
@@ -127,14 +141,12 @@ def _gradients(what, grads):
     return grads.dense(what, "gradients")
 
 
-@torch.no_grad()
 def grad_norm(grads):
     """The 2-norm of all gradients as if they were one vector: a float32 scalar on their device.  Sums in 64 bits."""
     grads = _gradients("grad_norm", grads)
     return _norm_and_factor(grads, math.inf)[0] if len(grads) else torch.zeros(())
 
 
-@torch.no_grad()
 def clip_grads_(grads, max_norm):
     """Scale all gradients in place by min(1, max_norm / (norm + 1e-6)) and return their norm before that (float32 scalar on their
     device).  Gradients within the limit are not written.  Mixed float32 / bfloat16 / float16 tensors are one vector."""
@@ -143,8 +155,8 @@ def clip_grads_(grads, max_norm):
     if not len(grads):
         return torch.zeros(())
     out = _norm_and_factor(grads, max_norm)
-    with torch.cuda.device(out.device):
-        check(_lib.lib().dtt_grad_scale(len(grads), grads.ptrs, grads.counts, grads.types, out.data_ptr() + 4, stream_ptr(out.device)), "grad_scale")
+    with _on(grads.device):
+        check(_lib.lib().dtt_grad_scale(len(grads), grads.ptrs, grads.counts, grads.types, out.data_ptr() + 4, _stream(grads.device)), "grad_scale")
     _written(grads.tensors)
     return out[0]
 
@@ -160,7 +172,7 @@ def clip_grad_norm_(parameters, max_norm):
         if g is None:
             continue
         if g.layout == torch.strided and not _dense(g):
-            g = p.grad = g.contiguous()
+            g = p.grad = g.detach().contiguous()
         grads.append(g)
     return clip_grads_(grads, max_norm)
 
@@ -227,7 +239,8 @@ class _Step:
             if at & 1 == 0:
                 raise ValueError("%s: a gradient has its parameter's shape (got %s for %s)" % (what, tuple(y.shape), tuple(x.shape)))
             # a gradient in another order of its dimensions (or an expanded one) is brought into the parameter's
-            lists[1] = [y if x.shape != y.shape or _same_order(x, y) else torch.empty_like(x).copy_(y) for x, y in zip(lists[0], lists[1])]
+            with torch.no_grad():
+                lists[1] = [y if x.shape != y.shape or _same_order(x, y) else torch.empty_like(x).copy_(y) for x, y in zip(lists[0], lists[1])]
             g = _List(what, lists[1])
             at = _tensorlist().differ(lists[0], lists[1])
         if s.type != 0 or s.counts != _ONE * n:
@@ -244,8 +257,14 @@ class _Step:
                 t, q = x.tensors[at >> 1], lists[0][at >> 1]
                 raise ValueError("%s: moments have their parameter's shape and memory order (got %s, strides %s for %s, strides %s)" %
                                  (what, tuple(t.shape), t.stride(), tuple(q.shape), q.stride()))
+        self.max_norm = -1.0
         if clip is None and (max_norm is not None or self.skip_nonfinite):
-            clip = _norm_and_factor(g, math.inf if max_norm is None else max_norm)
+            max_norm = math.inf if max_norm is None else max_norm
+            if p.type >= 0:      # one call: the library computes the norm on its way
+                self.max_norm = max_norm
+                clip = torch.empty(2, dtype=torch.float32, device=lists[0][0].device)
+            else:
+                clip = _norm_and_factor(g, max_norm)
         self.params, self.grads, self.steps, self.moments, self.clip = p, g, s, m, clip
 
     def launch(self, call):
@@ -265,17 +284,16 @@ class _Step:
                                None if self.rates is None else array("Q", [self.rates[i] for i in at]), array("d", [self.decay[i] for i in at]), at))
         L = _lib.lib()
         device = self.params.tensors[0].device
-        with torch.cuda.device(device):
+        with _on(self.dev):
             for dtype, parts, lr, rates, decay, at in groups:
-                nbytes = L.dtt_adamw_workspace_bytes(len(parts[0]))
+                nbytes = L.dtt_adamw_workspace_bytes(len(parts[0]), parts[0].counts)
                 ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
                 call(L, len(parts[0]), dtype, [x.ptrs for x in parts], parts[0].counts, lr.tobytes(), None if rates is None else rates.tobytes(),
-                     decay.tobytes(), at, (ptr(self.clip), int(self.skip_nonfinite), ptr(ws), nbytes, stream_ptr(device)))
+                     decay.tobytes(), at, (self.max_norm, None if self.clip is None else self.clip.data_ptr(), int(self.skip_nonfinite), ws.data_ptr(), nbytes, _stream(self.dev)))
         _written(*[x.tensors for x in [self.params, self.steps] + self.moments])
         return None if self.clip is None else self.clip[0]
 
 
-@torch.no_grad()
 def adamw_(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None,
            skip_nonfinite=False, clip=None):
     """One AdamW step of all tensors, in place.  Per tensor t <- t + 1 in its step counter (one float32), then
@@ -300,7 +318,6 @@ def blocks_of(numel):
     return (numel + BLOCK - 1) // BLOCK
 
 
-@torch.no_grad()
 def adamw8_(params, grads, exp_avgs, exp_avg_sqs, bases, steps, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None,
             skip_nonfinite=False, clip=None, seed=0, ids=None):
     """adamw_ with the moments in 8 bits: exp_avgs / exp_avg_sqs are uint8 codes in the parameters' shape and memory order, bases int16
@@ -343,7 +360,6 @@ def _check_bases(what, like, bases, dev):
         raise ValueError("%s: all tensors must be on one device" % what)
 
 
-@torch.no_grad()
 def unpack_moments_(exp_avgs, exp_avg_sqs, bases, out_avgs, out_avg_sqs):
     """Write the values that 8-bit moments stand for into out_avgs / out_avg_sqs (all float32 or all bfloat16, which holds them exactly;
     in the codes' shape and memory order)."""
@@ -364,8 +380,8 @@ def unpack_moments_(exp_avgs, exp_avg_sqs, bases, out_avgs, out_avg_sqs):
         raise ValueError("%s: codes and values have one shape and memory order" % what)
     dev = _device_of(what, [m, v, x, y])
     _check_bases(what, m, b, dev)
-    with torch.cuda.device(dev):
-        check(_lib.lib().dtt_adamw8_unpack(n, m.ptrs, v.ptrs, b.ptrs, m.counts, x.type, x.ptrs, y.ptrs, stream_ptr(dev)), what)
+    with _on(dev):
+        check(_lib.lib().dtt_adamw8_unpack(n, m.ptrs, v.ptrs, b.ptrs, m.counts, x.type, x.ptrs, y.ptrs, _stream(dev)), what)
     _written(lists[3], lists[4])
 
 

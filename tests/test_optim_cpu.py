@@ -158,24 +158,24 @@ def test_library_refuses_bad_arguments_without_a_gpu():
     assert L.dtt_grad_scale(1, P(base), N(8), I(0), None, None) == 0 and "null" in _lib.last_error()
 
     def step(p=(base, base + 64), g=(base + 128, base + 192), m=(base + 256, base + 320), v=(base + 384, base + 448), s=(base + 512, base + 516),
-             n=(16, 16), dtype=0, lr=(1e-3, 1e-3), wd=(0.0, 0.0), b1=0.9, b2=0.999, eps=1e-8, clip=None, skip=0, w=ws, wb=4096):
-        return L.dtt_adamw_step(2, dtype, P(*p), P(*g), P(*m), P(*v), N(*n), P(*s), D(*lr), None, D(*wd), b1, b2, eps, clip, skip, w, wb, None)
+             n=(16, 16), dtype=0, lr=(1e-3, 1e-3), wd=(0.0, 0.0), b1=0.9, b2=0.999, eps=1e-8, limit=-1.0, clip=None, skip=0, w=ws, wb=4096):
+        return L.dtt_adamw_step(2, dtype, P(*p), P(*g), P(*m), P(*v), N(*n), P(*s), D(*lr), None, D(*wd), b1, b2, eps, limit, clip, skip, w, wb, None)
     for kw, why in ((dict(p=(base, base)), "share memory"), (dict(m=(base + 256, base + 260)), "share memory"), (dict(g=(base + 4, base + 192)), "share memory"),
                     (dict(s=(base + 512, base + 512)), "share memory"), (dict(s=(base + 512, None)), "step counter"), (dict(p=(base + 1, base + 64)), "unaligned"),
                     (dict(v=(base + 384, None)), "moment"), (dict(dtype=5), "element type"), (dict(b1=1.0), "betas"), (dict(b2=-0.1), "betas"),
                     (dict(b2=float("nan")), "betas"), (dict(eps=-1.0), "eps"), (dict(lr=(1e-3, -1.0)), "learning rate"), (dict(wd=(float("nan"), 0.0)), "weight decay"),
-                    (dict(skip=1), "norm"), (dict(wb=8), "workspace"), (dict(w=ws + 4), "workspace"), (dict(n=(16, -3)), "element count")):
+                    (dict(skip=1), "norm and factor"), (dict(limit=1.0), "norm and factor"), (dict(limit=float("nan")), "not a number"), (dict(wb=8), "workspace"), (dict(w=ws + 4), "workspace"), (dict(n=(16, -3)), "element count")):
         assert step(**kw) == 0 and why in _lib.last_error(), (kw, _lib.last_error())
 
     def step8(m=(base + 256,), v=(base + 320,), b=(base + 512,), n=(16,), p=(base,), g=(base + 128,), s=(base + 600,)):
-        return L.dtt_adamw8_step(1, 0, P(*p), P(*g), P(*m), P(*v), P(*b), N(*n), P(*s), D(1e-3), None, D(0.0), None, 0, 0.9, 0.999, 1e-8, None, 0, ws,
+        return L.dtt_adamw8_step(1, 0, P(*p), P(*g), P(*m), P(*v), P(*b), N(*n), P(*s), D(1e-3), None, D(0.0), None, 0, 0.9, 0.999, 1e-8, -1.0, None, 0, ws,
                                  4096, None)
     for kw, why in ((dict(m=(base + 256,), v=(base + 260,)), "share memory"), (dict(b=(base + 513,)), "unaligned"), (dict(b=(None,)), "null"),
                     (dict(b=(base + 256,)), "share memory"), (dict(m=(None,)), "null")):
         assert step8(**kw) == 0 and why in _lib.last_error(), (kw, _lib.last_error())
     assert L.dtt_adamw8_unpack(1, P(base), P(base + 64), P(base + 128), N(16), 2, P(base + 256), P(base + 512), None) == 0 and "fp16" in _lib.last_error()
     assert L.dtt_adamw8_unpack(1, P(base), P(base + 64), P(base + 128), N(16), 0, P(base + 256), P(base + 300), None) == 0 and "share memory" in _lib.last_error()
-    assert L.dtt_adamw_workspace_bytes(10) >= 160 and L.dtt_grad_norm_workspace_bytes(0, None) > 0
+    assert L.dtt_adamw_workspace_bytes(2, N(4, 4)) >= 40 and L.dtt_grad_norm_workspace_bytes(0, None) > 0
 
 
 def test_optimizer_choice_and_groups():
