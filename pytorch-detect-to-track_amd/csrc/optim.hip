@@ -21,20 +21,22 @@ constexpr int kMaxStep8 = 72;     // 6 * 8 + 4
 constexpr int kMaxPrepare = 280;  // 8 + 4 + 1, and kMaxRates different rates
 constexpr int kMaxRates = 8;
 constexpr int kNormWorkgroups = 2048;   // 8 on a CU: all resident at once
-constexpr long kMaxNumel = 1L << 34;   // element / 8 fits the 32-bit hash input; a launch's workgroups (kMaxNumel / 4096 * kMax*) fit an int
+constexpr long kMaxNumel = 1L << 34;   // element / 8 fits the 32-bit hash input; a launch's workgroups (kMaxNumel / 2048 * kMax*) fit an int
 
 enum { kF32 = 0, kBf16 = 1, kF16 = 2 };
 
 // ------------------------------------------------------------------------------------------------ element types
 // Vector accesses at ELEMENT alignment: views of a flat bucket start anywhere, and the memory pipe takes wide accesses at any
-// element boundary (a line that is cut costs a second request, nothing else).
+// element boundary (a line that is cut costs a second request, nothing else).  All of them are non-temporal: every byte of a step is
+// used once, and lines that are not kept leave the memory-side cache to the gradients that the norm has just read (Res-101's clipped
+// step 350 -> 316 us, the norm of 1.2 G bf16 422 -> 380 us = 6.4 TB/s).
 template <typename T, int N> struct Wide {
   typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
 };
 
 template <typename T, int N> __device__ __forceinline__ void load_f32(const T* p, float (&x)[N]) {
   typedef typename Wide<T, N>::type V;
-  const V v = *reinterpret_cast<const V*>(p);
+  const V v = __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = (float)v[i];
 }
@@ -43,7 +45,7 @@ template <typename T, int N> __device__ __forceinline__ void store_f32(T* p, con
   V v;
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = (T)x[i];   // round to nearest even
-  *reinterpret_cast<V*>(p) = v;
+  __builtin_nontemporal_store(v, reinterpret_cast<V*>(p));
 }
 
 // index of the tensor that owns this workgroup: block0[0 .. n] are prefix sums in the kernel arguments.  The lanes compare 64
@@ -245,11 +247,25 @@ struct Consts {
   float beta1, one_beta1, beta2, one_beta2, eps;
 };
 
+// The quotient of the update for 8-bit moments, whose kernel has about as many instructions as it has bytes: v_sqrt and v_rcp, each good
+// to 2^-24, in place of the exactly rounded sequences (302 M bf16: step and unpacking 985 -> 884 us).  v_sqrt takes a v below 2^-126 for 0:
+// beside eps >= 2^-32 that is below 2^-24 of the denominator (root is at most 2^7 for beta2 <= 0.9999); a smaller eps takes the exact
+// sequences (a uniform branch).
+__device__ __forceinline__ float quotient8(float m, float v, float root, float eps) {
+  if (eps < 0x1p-32f) return m / (sqrtf(v) * root + eps);
+  return m * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v) * root + eps);
+}
+
 // m <- beta1 m + (1 - beta1) g;  v <- beta2 v + (1 - beta2) g^2;  p <- keep p - size * m / (root sqrt(v) + eps)
 __device__ __forceinline__ void adamw_element(float& p, float g, float& m, float& v, const Consts& k, const Factors& f) {
   m = m * k.beta1 + g * k.one_beta1;
   v = v * k.beta2 + (g * g) * k.one_beta2;
   p = p * f.keep - (m / (sqrtf(v) * f.root + k.eps)) * f.size;
+}
+__device__ __forceinline__ void adamw8_element(float& p, float g, float& m, float& v, const Consts& k, const Factors& f) {
+  m = m * k.beta1 + g * k.one_beta1;
+  v = v * k.beta2 + (g * g) * k.one_beta2;
+  p = p * f.keep - quotient8(m, v, f.root, k.eps) * f.size;
 }
 
 // ------------------------------------------------------------------------------------------------ AdamW, 32-bit moments
@@ -262,11 +278,26 @@ struct StepTable {
   int block0[kMaxStep];
   int n;
 };
-constexpr int kStepElems = kThreads * 16;   // elements per workgroup
+// Elements per thread, four neighbours at a time: all loads of a thread are issued before its first store (the compiler may not move a
+// load over a store to memory it cannot tell apart), and a wave's accesses are runs of 1 KiB of fp32.  Measured on MI355X, clipped
+// Res-101 fp32 / 604 M bf16, us: one group of four in flight 324 / 2408, two 316 / 2356, four 304 / 2290 (5.8 TB/s), eight 313 / 2420;
+// workgroups of 8 elements per thread and fp32 299, bf16 2350.  Eight neighbours per lane (one 16-byte access of bf16, two of its
+// moments 32 bytes apart): 2560.
+template <typename T> struct StepShape {
+  static constexpr int kGroups = sizeof(T) == 4 ? 2 : 4;
+  static constexpr int kElems = kThreads * 4 * kGroups;   // per workgroup
+};
+// Elements in front of the first 128-byte boundary of m: the first workgroup takes them one by one, so that the runs of a view into a
+// flat buffer -- whose four tensors usually start alike -- do not cut lines.
+__host__ __device__ __forceinline__ int step_head(const float* m, long numel) {
+  const long h = (32 - (long)((reinterpret_cast<uintptr_t>(m) >> 2) & 31)) & 31;
+  return (int)(h < numel ? h : numel);
+}
 
-template <typename T, int N>
+template <typename T>
 __global__ __launch_bounds__(kThreads) void adamw_step_kernel(StepTable tab, const Factors* __restrict__ factors,
                                                               const float* __restrict__ clip, int skip_nonfinite, Consts k) {
+  constexpr int N = 4, U = StepShape<T>::kGroups;
   const int i = owner(tab.block0, tab.n, blockIdx.x);
   if (clip && skipped(clip, skip_nonfinite)) return;
   const float c = clip ? clip[1] : 1.f;
@@ -276,26 +307,50 @@ __global__ __launch_bounds__(kThreads) void adamw_step_kernel(StepTable tab, con
   float* m = tab.m[i];
   float* v = tab.v[i];
   const long numel = tab.numel[i];
-  long e = (long)((int)blockIdx.x - tab.block0[i]) * kStepElems + (long)threadIdx.x * N;
+  const int head = step_head(m, numel);
+  const int block = (int)blockIdx.x - tab.block0[i];
+  const auto single = [&](long q) {
+    float xp = (float)p[q], xm = m[q], xv = v[q];
+    adamw_element(xp, (float)g[q] * c, xm, xv, k, f);
+    p[q] = (T)xp; m[q] = xm; v[q] = xv;
+  };
+  if (block == 0 && (int)threadIdx.x < head) single(threadIdx.x);
+  const long e0 = head + (long)block * StepShape<T>::kElems;
+  const long e = e0 + (long)threadIdx.x * N;
+  if (e0 + StepShape<T>::kElems <= numel) {
+    float xp[U][N], xg[U][N], xm[U][N], xv[U][N];
 #pragma unroll
-  for (int u = 0; u < kStepElems / (kThreads * N); ++u, e += kThreads * N) {
-    if (e + N <= numel) {
+    for (int u = 0; u < U; ++u) {
+      load_f32<T, N>(g + e + u * kThreads * N, xg[u]);
+      load_f32<float, N>(m + e + u * kThreads * N, xm[u]);
+      load_f32<float, N>(v + e + u * kThreads * N, xv[u]);
+      load_f32<T, N>(p + e + u * kThreads * N, xp[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) adamw_element(xp[u][j], xg[u][j] * c, xm[u][j], xv[u][j], k, f);
+      store_f32<T, N>(p + e + u * kThreads * N, xp[u]);
+      store_f32<float, N>(m + e + u * kThreads * N, xm[u]);
+      store_f32<float, N>(v + e + u * kThreads * N, xv[u]);
+    }
+    return;
+  }
+  for (int u = 0; u < U; ++u) {   // the end of a tensor
+    const long q = e + u * kThreads * N;
+    if (q + N <= numel) {
       float xp[N], xg[N], xm[N], xv[N];
-      load_f32<T, N>(p + e, xp);
-      load_f32<T, N>(g + e, xg);
-      load_f32<float, N>(m + e, xm);
-      load_f32<float, N>(v + e, xv);
+      load_f32<T, N>(g + q, xg);
+      load_f32<float, N>(m + q, xm);
+      load_f32<float, N>(v + q, xv);
+      load_f32<T, N>(p + q, xp);
 #pragma unroll
       for (int j = 0; j < N; ++j) adamw_element(xp[j], xg[j] * c, xm[j], xv[j], k, f);
-      store_f32<T, N>(p + e, xp);
-      store_f32<float, N>(m + e, xm);
-      store_f32<float, N>(v + e, xv);
+      store_f32<T, N>(p + q, xp);
+      store_f32<float, N>(m + q, xm);
+      store_f32<float, N>(v + q, xv);
     } else {
-      for (long q = e; q < numel && q < e + N; ++q) {
-        float xp = (float)p[q], xm = m[q], xv = v[q];
-        adamw_element(xp, (float)g[q] * c, xm, xv, k, f);
-        p[q] = (T)xp; m[q] = xm; v[q] = xv;
-      }
+      for (long r = q; r < numel; ++r) single(r);
     }
   }
 }
@@ -444,7 +499,7 @@ __global__ __launch_bounds__(kThreads) void adamw8_step_kernel(Step8Table tab, c
       float xm[4], xv[4];
       decode4(um[u], uv[u], b[u], xm, xv);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) adamw_element(xp[u][j], xg[u][j] * c, xm[j], xv[j], k, f);
+      for (int j = 0; j < 4; ++j) adamw8_element(xp[u][j], xg[u][j] * c, xm[j], xv[j], k, f);
       store_f32<T, 4>(p + e + u * kBlock, xp[u]);
       const unsigned h = mix32((unsigned)((e + u * kBlock) >> 3) ^ f.key);
       unsigned q[4];
@@ -472,7 +527,7 @@ __global__ __launch_bounds__(kThreads) void adamw8_step_kernel(Step8Table tab, c
         xm[j] = decode_m(cm[e1 + j], b & 0xFFFF);
         xv[j] = decode_v(cv[e1 + j], b >> 16);
         float xp = (float)p[e1 + j];
-        adamw_element(xp, (float)g[e1 + j] * c, xm[j], xv[j], k, f);
+        adamw8_element(xp, (float)g[e1 + j] * c, xm[j], xv[j], k, f);
         p[e1 + j] = (T)xp;
       }
     }
@@ -805,14 +860,16 @@ extern "C" int dtt_adamw_step(int n, int dtype, void* const* params, const void*
       const int i = i0 + j;
       tab.p[j] = params[i]; tab.g[j] = grads[i]; tab.m[j] = exp_avgs[i]; tab.v[j] = exp_avg_sqs[i]; tab.numel[j] = numel[i];
       tab.block0[j] = blocks;
-      const long nb = (numel[i] + kStepElems - 1) / kStepElems;
+      const int per = dtype == kF32 ? StepShape<float>::kElems : StepShape<__bf16>::kElems;
+      const long body = numel[i] - step_head(exp_avgs[i], numel[i]);
+      const long nb = numel[i] == 0 ? 0 : body <= per ? 1 : (body + per - 1) / per;
       blocks += (int)nb;
     }
     if (blocks == 0) continue;
     const dim3 grid((unsigned)blocks), wg(kThreads);
-    if (dtype == kF32) hipLaunchKernelGGL((adamw_step_kernel<float, 4>), grid, wg, 0, stream, tab, factors + i0, clip, skip_nonfinite, k);
-    else if (dtype == kBf16) hipLaunchKernelGGL((adamw_step_kernel<__bf16, 8>), grid, wg, 0, stream, tab, factors + i0, clip, skip_nonfinite, k);
-    else hipLaunchKernelGGL((adamw_step_kernel<_Float16, 8>), grid, wg, 0, stream, tab, factors + i0, clip, skip_nonfinite, k);
+    if (dtype == kF32) hipLaunchKernelGGL((adamw_step_kernel<float>), grid, wg, 0, stream, tab, factors + i0, clip, skip_nonfinite, k);
+    else if (dtype == kBf16) hipLaunchKernelGGL((adamw_step_kernel<__bf16>), grid, wg, 0, stream, tab, factors + i0, clip, skip_nonfinite, k);
+    else hipLaunchKernelGGL((adamw_step_kernel<_Float16>), grid, wg, 0, stream, tab, factors + i0, clip, skip_nonfinite, k);
     DTT_CHECK_LAUNCH("adamw_step_kernel");
   }
   dtt_prof_end("adamw", stream);
