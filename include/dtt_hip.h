@@ -38,7 +38,7 @@ const char* dtt_last_error(void);
  * correlation: band kernel + the streamed launch; phase 2 alone when the op is issued in phases, whose phase 1 is "corr_bwd_band"),
  * "proposal_op" (the proposal layer of all images of a call, "nms_op" inside it: both NMS phases), "anchor_target_op",
  * "rpn_loss" (forward of both RPN losses), "psroi_pm_bwd" (the one-launch PSRoI backward of a map's heads), "grad_norm",
- * "grad_scale", "adamw", "adamw8" (all launches of one call);
+ * "grad_clip", "adamw", "adamw8" (all launches of one call);
  * kernels: "corr_nhwc" (corr_wsplit_kernel), "corr_fwd_mfma" /
  * "corr_fwd_reduce" (the NCHW pair), "head_gemm", "rpn_head_gemm", "psroi_pm" (position-major poolings), "psroi_fwd_plane",
  * "nms_mask", "nms_sweep", "proposal_select_sort".  tag = NULL detaches.  Events are hipEvent_t handles owned
@@ -600,11 +600,12 @@ int dtt_tube_link(const float* dets, int det_stride, const int* n, const float* 
  * dtt_grad_norm: out[0] = sqrt(sum of all squares), out[1] = min(1, max_norm / (out[0] + 1e-6)) -- the factor that brings the
  * gradients to the limit; max_norm = infinity asks for the norm alone (factor 1).  Squares and sums in 64 bits, in a fixed order.
  * workspace: dtt_grad_norm_workspace_bytes(n, numel) bytes, 8-byte aligned.
- * dtt_grad_scale: grads *= *factor (device scalar); a factor of 1 leaves them untouched. */
+ * dtt_grad_clip: the same, and grads *= out[1]; a factor of 1 leaves them untouched. */
 size_t dtt_grad_norm_workspace_bytes(int n, const long* numel);
 int dtt_grad_norm(int n, const void* const* grads, const long* numel, const int* dtypes, double max_norm, float* out,
                   void* workspace, size_t workspace_bytes, void* stream);
-int dtt_grad_scale(int n, void* const* grads, const long* numel, const int* dtypes, const float* factor, void* stream);
+int dtt_grad_clip(int n, void* const* grads, const long* numel, const int* dtypes, double max_norm, float* out, void* workspace,
+                  size_t workspace_bytes, void* stream);
 /* One AdamW step (decoupled weight decay) of n tensors of one dtype.  Per tensor: t = ++*step;  g *= clip[1];  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;
  * p = p (1 - lr decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps).   Moments fp32, arithmetic fp32, factors of
  * t in 64 bits; p rounded once to its dtype.  max_norm >= 0: the call computes norm and factor of its gradients as dtt_grad_norm

@@ -21,7 +21,7 @@ constexpr int kMaxStep8 = 72;     // 6 * 8 + 4
 constexpr int kMaxPrepare = 280;  // 8 + 4 + 1, and kMaxRates different rates
 constexpr int kMaxRates = 8;
 constexpr int kNormWorkgroups = 2048;   // 8 on a CU: all resident at once
-constexpr long kMaxNumel = 1L << 34;   // element / 8 fits the 32-bit hash input; a launch's workgroups (kMaxNumel / 2048 * kMax*) fit an int
+constexpr long kMaxNumel = 1L << 34;   // element / 8 fits the 32-bit hash input; a launch's workgroups (kMaxNumel / 1024 * kMax*) fit an int
 
 enum { kF32 = 0, kBf16 = 1, kF16 = 2 };
 
@@ -129,21 +129,27 @@ __global__ __launch_bounds__(kThreads) void grad_norm_kernel(NormTable tab, doub
 }
 
 // The partial sums of all workgroups, in index order within a thread, then over the threads: norm and factor, in every thread.
-constexpr int kFinish = 512;   // threads
-__device__ __forceinline__ float2 finish_norm(const double* __restrict__ partial, int n, double max_norm) {
+constexpr int kFinish = 512;   // threads of the launches that do nothing else at length
+template <int NT> __device__ __forceinline__ float2 finish_norm(const double* __restrict__ partial, int n, double max_norm) {
   double s = 0.0;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < n; i += kFinish) s += partial[i];
-  s = workgroup_sum<kFinish / 64>(s);
+#pragma unroll 8
+  for (int i = threadIdx.x; i < n; i += NT) s += partial[i];
+  s = workgroup_sum<NT / 64>(s);
   const double norm = sqrt(s);
   // (an infinite limit asks for the norm alone; a norm that is not a number stays one in the factor, an infinite one gives 0)
   const double f = max_norm / (norm + 1e-6);
   return make_float2((float)norm, isinf(max_norm) ? 1.f : f < 1.0 || f != f ? (float)f : 1.f);
 }
 
+struct NormPart {
+  const double* partial;   // NULL: the norm is not this call's to compute
+  int n;
+  double max_norm;
+};
+
 __global__ __launch_bounds__(kFinish) void grad_norm_finish_kernel(const double* __restrict__ partial, int n, double max_norm,
                                                                    float* __restrict__ out) {
-  const float2 r = finish_norm(partial, n, max_norm);
+  const float2 r = finish_norm<kFinish>(partial, n, max_norm);
   if (threadIdx.x == 0) { out[0] = r.x; out[1] = r.y; }
 }
 
@@ -158,8 +164,20 @@ struct ScaleTable {
 };
 
 template <typename T, int N> __device__ __forceinline__ void scale_run(T* g, long e0, long e1, float f) {
+  constexpr int kFly = 4;
   long e = e0 + (long)threadIdx.x * N;
-  for (; e + N <= e1; e += (long)kThreads * N) {
+  for (; e + (kFly - 1) * kThreads * N + N <= e1; e += kFly * kThreads * N) {
+    float x[kFly][N];
+#pragma unroll
+    for (int u = 0; u < kFly; ++u) load_f32<T, N>(g + e + u * kThreads * N, x[u]);
+#pragma unroll
+    for (int u = 0; u < kFly; ++u) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[u][i] *= f;
+      store_f32<T, N>(g + e + u * kThreads * N, x[u]);
+    }
+  }
+  for (; e + N <= e1; e += kThreads * N) {
     float x[N];
     load_f32<T, N>(g + e, x);
 #pragma unroll
@@ -169,8 +187,12 @@ template <typename T, int N> __device__ __forceinline__ void scale_run(T* g, lon
   for (; e < e1; ++e) g[e] = (T)((float)g[e] * f);
 }
 
-__global__ __launch_bounds__(kThreads) void grad_scale_kernel(ScaleTable tab, const float* __restrict__ factor) {
-  const float f = *factor;
+// Every workgroup joins the partial sums itself (16 KiB of L2 at most): a launch of one workgroup in between would keep the device
+// waiting for 7 us.
+__global__ __launch_bounds__(kThreads) void grad_clip_kernel(ScaleTable tab, NormPart part, float* __restrict__ out) {
+  const float2 r = finish_norm<kThreads>(part.partial, part.n, part.max_norm);
+  if (out && blockIdx.x == 0 && threadIdx.x == 0) { out[0] = r.x; out[1] = r.y; }
+  const float f = r.y;
   if (f == 1.f) return;   // within the limit: the gradients are neither read nor written
   const int i = owner(tab.block0, tab.n, blockIdx.x);
   const long e0 = (long)((int)blockIdx.x - tab.block0[i]) * tab.chunk;
@@ -199,11 +221,6 @@ struct PrepareTable {
   unsigned seed;
   double beta1, beta2;
 };
-struct NormPart {
-  const double* partial;   // NULL: the call does not compute a norm, clip (or NULL) is given
-  int n;
-  double max_norm;
-};
 struct Factors {
   float keep, size, root;
   unsigned key;
@@ -223,7 +240,7 @@ __global__ __launch_bounds__(kFinish) void adamw_prepare_kernel(PrepareTable tab
                                                                 Factors* __restrict__ factors) {
   bool skip = false;
   if (part.partial) {
-    const float2 r = finish_norm(part.partial, part.n, part.max_norm);
+    const float2 r = finish_norm<kFinish>(part.partial, part.n, part.max_norm);
     if (threadIdx.x == 0) { clip[0] = r.x; clip[1] = r.y; }
     skip = skip_nonfinite && !isfinite(r.x);
   } else if (clip) {
@@ -278,15 +295,11 @@ struct StepTable {
   int block0[kMaxStep];
   int n;
 };
-// Elements per thread, four neighbours at a time: all loads of a thread are issued before its first store (the compiler may not move a
-// load over a store to memory it cannot tell apart), and a wave's accesses are runs of 1 KiB of fp32.  Measured on MI355X, clipped
-// Res-101 fp32 / 604 M bf16, us: one group of four in flight 324 / 2408, two 316 / 2356, four 304 / 2290 (5.8 TB/s), eight 313 / 2420;
-// workgroups of 8 elements per thread and fp32 299, bf16 2350.  Eight neighbours per lane (one 16-byte access of bf16, two of its
-// moments 32 bytes apart): 2560.
-template <typename T> struct StepShape {
-  static constexpr int kGroups = sizeof(T) == 4 ? 2 : 4;
-  static constexpr int kElems = kThreads * 4 * kGroups;   // per workgroup
-};
+// A thread takes four neighbours and nothing else: a wave's accesses are runs of 1 KiB of fp32, and the workgroups in flight walk one
+// compact window of each buffer.  Measured on MI355X, clipped Res-101 fp32 / 604 M bf16, us: one group of four 297 / 2165 (6.1 TB/s);
+// two groups, loads first, 299 / 2345; four 304 / 2299; four, each loaded behind the one before it, 324 / 2408.  Eight neighbours of
+// bf16 (one 16-byte access, two of the moments 32 bytes apart): 2560.
+constexpr int kStepElems = kThreads * 4;   // per workgroup
 // Elements in front of the first 128-byte boundary of m: the first workgroup takes them one by one, so that the runs of a view into a
 // flat buffer -- whose four tensors usually start alike -- do not cut lines.
 __host__ __device__ __forceinline__ int step_head(const float* m, long numel) {
@@ -297,7 +310,7 @@ __host__ __device__ __forceinline__ int step_head(const float* m, long numel) {
 template <typename T>
 __global__ __launch_bounds__(kThreads) void adamw_step_kernel(StepTable tab, const Factors* __restrict__ factors,
                                                               const float* __restrict__ clip, int skip_nonfinite, Consts k) {
-  constexpr int N = 4, U = StepShape<T>::kGroups;
+  constexpr int N = 4;
   const int i = owner(tab.block0, tab.n, blockIdx.x);
   if (clip && skipped(clip, skip_nonfinite)) return;
   const float c = clip ? clip[1] : 1.f;
@@ -315,43 +328,20 @@ __global__ __launch_bounds__(kThreads) void adamw_step_kernel(StepTable tab, con
     p[q] = (T)xp; m[q] = xm; v[q] = xv;
   };
   if (block == 0 && (int)threadIdx.x < head) single(threadIdx.x);
-  const long e0 = head + (long)block * StepShape<T>::kElems;
-  const long e = e0 + (long)threadIdx.x * N;
-  if (e0 + StepShape<T>::kElems <= numel) {
-    float xp[U][N], xg[U][N], xm[U][N], xv[U][N];
+  const long e = head + (long)block * kStepElems + (long)threadIdx.x * N;
+  if (e + N <= numel) {
+    float xp[N], xg[N], xm[N], xv[N];
+    load_f32<T, N>(g + e, xg);
+    load_f32<float, N>(m + e, xm);
+    load_f32<float, N>(v + e, xv);
+    load_f32<T, N>(p + e, xp);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      load_f32<T, N>(g + e + u * kThreads * N, xg[u]);
-      load_f32<float, N>(m + e + u * kThreads * N, xm[u]);
-      load_f32<float, N>(v + e + u * kThreads * N, xv[u]);
-      load_f32<T, N>(p + e + u * kThreads * N, xp[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) adamw_element(xp[u][j], xg[u][j] * c, xm[u][j], xv[u][j], k, f);
-      store_f32<T, N>(p + e + u * kThreads * N, xp[u]);
-      store_f32<float, N>(m + e + u * kThreads * N, xm[u]);
-      store_f32<float, N>(v + e + u * kThreads * N, xv[u]);
-    }
-    return;
-  }
-  for (int u = 0; u < U; ++u) {   // the end of a tensor
-    const long q = e + u * kThreads * N;
-    if (q + N <= numel) {
-      float xp[N], xg[N], xm[N], xv[N];
-      load_f32<T, N>(g + q, xg);
-      load_f32<float, N>(m + q, xm);
-      load_f32<float, N>(v + q, xv);
-      load_f32<T, N>(p + q, xp);
-#pragma unroll
-      for (int j = 0; j < N; ++j) adamw_element(xp[j], xg[j] * c, xm[j], xv[j], k, f);
-      store_f32<T, N>(p + q, xp);
-      store_f32<float, N>(m + q, xm);
-      store_f32<float, N>(v + q, xv);
-    } else {
-      for (long r = q; r < numel; ++r) single(r);
-    }
+    for (int j = 0; j < N; ++j) adamw_element(xp[j], xg[j] * c, xm[j], xv[j], k, f);
+    store_f32<T, N>(p + e, xp);
+    store_f32<float, N>(m + e, xm);
+    store_f32<float, N>(v + e, xv);
+  } else {
+    for (long r = e; r < numel; ++r) single(r);   // the end of a tensor
   }
 }
 
@@ -392,8 +382,13 @@ struct Step8Table {
   int block0[kMaxStep8];
   int n;
 };
-constexpr int kWaveBlocks = 4;                                       // blocks that a wave holds at a time
-constexpr int kStep8Elems = kThreads / 64 * kWaveBlocks * kBlock;    // elements per workgroup
+// Blocks that a wave holds at a time: four share what a workgroup does first (finding its tensor, pointers, factors), which costs
+// against the kernel's own instructions; a launch that would give the CUs less than four such workgroups each takes one block per wave
+// instead.  302 M bf16, step and unpacking: four 884 us, two 905, one 1190; 1.1 M fp32: step 9.0 / 7.3 / 6.8 us, unpacking 5.5 / 5.1 / 5.3;
+// 72 odd tensors of 1.2 M fp16 together: 10.4 / 7.5 / 6.3 us, unpacking 8.1 / 5.9 / 4.9.
+template <int WB> struct Wave8 {
+  static constexpr int kElems = kThreads / 64 * WB * kBlock;   // per workgroup
+};
 
 __device__ __forceinline__ unsigned max_halves(unsigned a, unsigned b) {
   typedef unsigned short Pair __attribute__((ext_vector_type(2)));
@@ -463,9 +458,9 @@ __device__ __forceinline__ void decode4(unsigned cm, unsigned cv, int base, floa
 
 typedef unsigned Word __attribute__((aligned(1)));   // four codes, at any address
 
-// A wave holds four blocks: a lane has four neighbours of each, so that all of the wave's accesses are runs of memory (1 KiB of fp32
+// A lane has four neighbours of each of the wave's blocks, so that all of the wave's accesses are runs of memory (1 KiB of fp32
 // parameters, 256 bytes of codes), and all loads are on their way before the first is used.
-template <typename T>
+template <typename T, int WB>
 __global__ __launch_bounds__(kThreads) void adamw8_step_kernel(Step8Table tab, const Factors* __restrict__ factors,
                                                                const float* __restrict__ clip, int skip_nonfinite, Consts k) {
   const int i = owner(tab.block0, tab.n, blockIdx.x);
@@ -478,16 +473,16 @@ __global__ __launch_bounds__(kThreads) void adamw8_step_kernel(Step8Table tab, c
   unsigned char* cv = tab.v[i];
   const long numel = tab.numel[i];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const long e0 = (long)((int)blockIdx.x - tab.block0[i]) * kStep8Elems + wave * (kWaveBlocks * kBlock);
+  const long e0 = (long)((int)blockIdx.x - tab.block0[i]) * Wave8<WB>::kElems + wave * (WB * kBlock);
   if (e0 >= numel) return;
   int* base = tab.base[i] + e0 / kBlock;
   const long e = e0 + lane * 4;
-  if (e0 + kWaveBlocks * kBlock <= numel) {
-    float xp[kWaveBlocks][4], xg[kWaveBlocks][4];
-    unsigned um[kWaveBlocks], uv[kWaveBlocks];
-    int b[kWaveBlocks];
+  if (e0 + WB * kBlock <= numel) {
+    float xp[WB][4], xg[WB][4];
+    unsigned um[WB], uv[WB];
+    int b[WB];
 #pragma unroll
-    for (int u = 0; u < kWaveBlocks; ++u) {
+    for (int u = 0; u < WB; ++u) {
       um[u] = *reinterpret_cast<const Word*>(cm + e + u * kBlock);
       uv[u] = *reinterpret_cast<const Word*>(cv + e + u * kBlock);
       load_f32<T, 4>(g + e + u * kBlock, xg[u]);
@@ -495,7 +490,7 @@ __global__ __launch_bounds__(kThreads) void adamw8_step_kernel(Step8Table tab, c
       b[u] = base[u];
     }
 #pragma unroll
-    for (int u = 0; u < kWaveBlocks; ++u) {
+    for (int u = 0; u < WB; ++u) {
       float xm[4], xv[4];
       decode4(um[u], uv[u], b[u], xm, xv);
 #pragma unroll
@@ -511,12 +506,12 @@ __global__ __launch_bounds__(kThreads) void adamw8_step_kernel(Step8Table tab, c
     }
     if (lane == 0) {
 #pragma unroll
-      for (int u = 0; u < kWaveBlocks; ++u) base[u] = b[u];
+      for (int u = 0; u < WB; ++u) base[u] = b[u];
     }
     return;
   }
   // the end of a tensor: elements behind it count as zeros of the block
-  for (int u = 0; u < kWaveBlocks && e0 + u * kBlock < numel; ++u) {
+  for (int u = 0; u < WB && e0 + u * kBlock < numel; ++u) {
     const long e1 = e + u * kBlock;
     const int b = base[u];
     float xm[4], xv[4];
@@ -557,11 +552,11 @@ struct UnpackTable {
   int n;
 };
 
-template <typename T> __global__ __launch_bounds__(kThreads) void unpack_moments_kernel(UnpackTable tab) {
+template <typename T, int WB> __global__ __launch_bounds__(kThreads) void unpack_moments_kernel(UnpackTable tab) {
   const int i = owner(tab.block0, tab.n, blockIdx.x);
   const long numel = tab.numel[i];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const long e0 = (long)((int)blockIdx.x - tab.block0[i]) * kStep8Elems + wave * (kWaveBlocks * kBlock);
+  const long e0 = (long)((int)blockIdx.x - tab.block0[i]) * Wave8<WB>::kElems + wave * (WB * kBlock);
   if (e0 >= numel) return;
   const int* base = tab.base[i] + e0 / kBlock;
   const long e = e0 + lane * 4;
@@ -569,17 +564,17 @@ template <typename T> __global__ __launch_bounds__(kThreads) void unpack_moments
   const unsigned char* cv = tab.v[i] + e;
   T* out_m = static_cast<T*>(tab.out_m[i]) + e;
   T* out_v = static_cast<T*>(tab.out_v[i]) + e;
-  if (e0 + kWaveBlocks * kBlock <= numel) {
-    unsigned um[kWaveBlocks], uv[kWaveBlocks];
-    int b[kWaveBlocks];
+  if (e0 + WB * kBlock <= numel) {
+    unsigned um[WB], uv[WB];
+    int b[WB];
 #pragma unroll
-    for (int u = 0; u < kWaveBlocks; ++u) {
+    for (int u = 0; u < WB; ++u) {
       um[u] = *reinterpret_cast<const Word*>(cm + u * kBlock);
       uv[u] = *reinterpret_cast<const Word*>(cv + u * kBlock);
       b[u] = base[u];
     }
 #pragma unroll
-    for (int u = 0; u < kWaveBlocks; ++u) {
+    for (int u = 0; u < WB; ++u) {
       float xm[4], xv[4];
       decode4(um[u], uv[u], b[u], xm, xv);
       store_f32<T, 4>(out_m + u * kBlock, xm);
@@ -587,7 +582,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void unpack_moments
     }
     return;
   }
-  for (int u = 0; u < kWaveBlocks && e0 + u * kBlock < numel; ++u)
+  for (int u = 0; u < WB && e0 + u * kBlock < numel; ++u)
     for (int j = 0; j < 4 && e + u * kBlock + j < numel; ++j) {
       out_m[u * kBlock + j] = (T)decode_m(cm[u * kBlock + j], base[u] & 0xFFFF);
       out_v[u * kBlock + j] = (T)decode_v(cv[u * kBlock + j], base[u] >> 16);
@@ -726,17 +721,31 @@ extern "C" int dtt_grad_norm(int n, const void* const* grads, const long* numel,
   return 1;
 }
 
-extern "C" int dtt_grad_scale(int n, void* const* grads, const long* numel, const int* dtypes, const float* factor, void* stream_) {
+extern "C" int dtt_grad_clip(int n, void* const* grads, const long* numel, const int* dtypes, double max_norm, float* out, void* workspace,
+                             size_t workspace_bytes, void* stream_) {
   hipStream_t stream = static_cast<hipStream_t>(stream_);
-  if (!check_grads("grad_scale", n, grads, numel, dtypes)) return 0;
-  DTT_REQUIRE(factor, "grad_scale: null pointer");
+  if (!check_grads("grad_clip", n, grads, numel, dtypes)) return 0;
+  DTT_REQUIRE(out && workspace && aligned_to(workspace, 8), "grad_clip: null or unaligned pointer");
+  DTT_REQUIRE(max_norm >= 0.0, "grad_clip: max_norm must not be negative");
+  DTT_REQUIRE(workspace_bytes >= dtt_grad_norm_workspace_bytes(n, numel), "grad_clip: workspace too small");
   Spans spans(n);
-  DTT_REQUIRE(spans.s, "grad_scale: out of host memory");
+  DTT_REQUIRE(spans.s, "grad_clip: out of host memory");
   for (int i = 0; i < n; ++i) spans.add(grads[i], numel[i] * type_bytes(dtypes[i]), true);
-  DTT_REQUIRE(!spans.clash(), "grad_scale: two gradients share memory");
+  DTT_REQUIRE(!spans.clash(), "grad_clip: two gradients share memory");
+  double* partial = static_cast<double*>(workspace);
+  dtt_prof_begin("grad_clip", stream);
+  NormPart part;
+  part.partial = partial;
+  part.max_norm = max_norm;
+  part.n = norm_partials(n, grads, numel, dtypes, 0, partial, stream);
+  if (part.n < 0) return 0;
+  if (part.n == 0) {   // nothing but empty tensors: norm 0
+    hipLaunchKernelGGL(grad_norm_finish_kernel, dim3(1), dim3(kFinish), 0, stream, partial, 0, max_norm, out);
+    DTT_CHECK_LAUNCH("grad_norm_finish_kernel");
+  }
   const long chunk = n > 0 ? norm_chunk(n, numel) : 1;
-  dtt_prof_begin("grad_scale", stream);
   ScaleTable tab;
+  float* to = out;
   for (int i = 0; i < n;) {
     tab.n = 0; tab.chunk = chunk;
     int here = 0;
@@ -747,10 +756,11 @@ extern "C" int dtt_grad_scale(int n, void* const* grads, const long* numel, cons
       here += (int)((numel[i] + chunk - 1) / chunk);
     }
     if (here == 0) break;
-    hipLaunchKernelGGL(grad_scale_kernel, dim3((unsigned)here), dim3(kThreads), 0, stream, tab, factor);
-    DTT_CHECK_LAUNCH("grad_scale_kernel");
+    hipLaunchKernelGGL(grad_clip_kernel, dim3((unsigned)here), dim3(kThreads), 0, stream, tab, part, to);
+    DTT_CHECK_LAUNCH("grad_clip_kernel");
+    to = nullptr;   // (the first launch has written norm and factor)
   }
-  dtt_prof_end("grad_scale", stream);
+  dtt_prof_end("grad_clip", stream);
   return 1;
 }
 
@@ -821,6 +831,17 @@ int prepare(int n, int dtype, const void* const* grads, const long* numel, float
   return 1;
 }
 
+// whether a launch over these tensors has waves hold four blocks (see Wave8)
+bool four_blocks(int n, const long* numel) {
+  long workgroups = 0;
+  for (int i = 0; i < n; ++i) workgroups += (numel[i] + Wave8<4>::kElems - 1) / Wave8<4>::kElems;
+  return workgroups >= 4L * dtt_device_cus();
+}
+int workgroups8(long numel, bool four) {
+  const int per = four ? Wave8<4>::kElems : Wave8<1>::kElems;
+  return (int)((numel + per - 1) / per);
+}
+
 Consts consts(double beta1, double beta2, double eps) {
   Consts k;
   k.beta1 = (float)beta1; k.one_beta1 = (float)(1.0 - beta1);
@@ -860,9 +881,8 @@ extern "C" int dtt_adamw_step(int n, int dtype, void* const* params, const void*
       const int i = i0 + j;
       tab.p[j] = params[i]; tab.g[j] = grads[i]; tab.m[j] = exp_avgs[i]; tab.v[j] = exp_avg_sqs[i]; tab.numel[j] = numel[i];
       tab.block0[j] = blocks;
-      const int per = dtype == kF32 ? StepShape<float>::kElems : StepShape<__bf16>::kElems;
       const long body = numel[i] - step_head(exp_avgs[i], numel[i]);
-      const long nb = numel[i] == 0 ? 0 : body <= per ? 1 : (body + per - 1) / per;
+      const long nb = numel[i] == 0 ? 0 : body <= kStepElems ? 1 : (body + kStepElems - 1) / kStepElems;
       blocks += (int)nb;
     }
     if (blocks == 0) continue;
@@ -902,19 +922,21 @@ extern "C" int dtt_adamw8_step(int n, int dtype, void* const* params, const void
   Step8Table tab;
   for (int i0 = 0; i0 < n; i0 += kMaxStep8) {
     tab.n = n - i0 < kMaxStep8 ? n - i0 : kMaxStep8;
+    const bool four = four_blocks(tab.n, numel + i0);
     int blocks = 0;
     for (int j = 0; j < tab.n; ++j) {
       const int i = i0 + j;
       tab.p[j] = params[i]; tab.g[j] = grads[i]; tab.m[j] = exp_avgs[i]; tab.v[j] = exp_avg_sqs[i]; tab.base[j] = reinterpret_cast<int*>(bases[i]);
       tab.numel[j] = numel[i]; tab.block0[j] = blocks;
-      const long nb = (numel[i] + kStep8Elems - 1) / kStep8Elems;
-      blocks += (int)nb;
+      blocks += workgroups8(numel[i], four);
     }
     if (blocks == 0) continue;
-    const dim3 grid((unsigned)blocks), wg(kThreads);
-    if (dtype == kF32) hipLaunchKernelGGL((adamw8_step_kernel<float>), grid, wg, 0, stream, tab, factors + i0, clip, skip_nonfinite, k);
-    else if (dtype == kBf16) hipLaunchKernelGGL((adamw8_step_kernel<__bf16>), grid, wg, 0, stream, tab, factors + i0, clip, skip_nonfinite, k);
-    else hipLaunchKernelGGL((adamw8_step_kernel<_Float16>), grid, wg, 0, stream, tab, factors + i0, clip, skip_nonfinite, k);
+    const auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kThreads), 0, stream, tab, factors + i0, clip, skip_nonfinite, k);
+    };
+    if (dtype == kF32) four ? launch(adamw8_step_kernel<float, 4>) : launch(adamw8_step_kernel<float, 1>);
+    else if (dtype == kBf16) four ? launch(adamw8_step_kernel<__bf16, 4>) : launch(adamw8_step_kernel<__bf16, 1>);
+    else four ? launch(adamw8_step_kernel<_Float16, 4>) : launch(adamw8_step_kernel<_Float16, 1>);
     DTT_CHECK_LAUNCH("adamw8_step_kernel");
   }
   dtt_prof_end("adamw8", stream);
@@ -945,18 +967,18 @@ extern "C" int dtt_adamw8_unpack(int n, const unsigned char* const* exp_avgs, co
   UnpackTable tab;
   for (int i0 = 0; i0 < n; i0 += kMaxStep8) {
     tab.n = n - i0 < kMaxStep8 ? n - i0 : kMaxStep8;
+    const bool four = four_blocks(tab.n, numel + i0);
     int blocks = 0;
     for (int j = 0; j < tab.n; ++j) {
       const int i = i0 + j;
-      tab.m[j] = exp_avgs[i]; tab.v[j] = exp_avg_sqs[i]; tab.base[j] = reinterpret_cast<const int*>(bases[i]); tab.out_m[j] = out_avgs[i]; tab.out_v[j] = out_avg_sqs[i];
-      tab.numel[j] = numel[i]; tab.block0[j] = blocks;
-      const long nb = (numel[i] + kStep8Elems - 1) / kStep8Elems;
-      blocks += (int)nb;
+      tab.m[j] = exp_avgs[i]; tab.v[j] = exp_avg_sqs[i]; tab.base[j] = reinterpret_cast<const int*>(bases[i]); tab.out_m[j] = out_avgs[i];
+      tab.out_v[j] = out_avg_sqs[i]; tab.numel[j] = numel[i]; tab.block0[j] = blocks;
+      blocks += workgroups8(numel[i], four);
     }
     if (blocks == 0) continue;
-    const dim3 grid((unsigned)blocks), wg(kThreads);
-    if (out_dtype == kF32) hipLaunchKernelGGL((unpack_moments_kernel<float>), grid, wg, 0, stream, tab);
-    else hipLaunchKernelGGL((unpack_moments_kernel<__bf16>), grid, wg, 0, stream, tab);
+    const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kThreads), 0, stream, tab); };
+    if (out_dtype == kF32) four ? launch(unpack_moments_kernel<float, 4>) : launch(unpack_moments_kernel<float, 1>);
+    else four ? launch(unpack_moments_kernel<__bf16, 4>) : launch(unpack_moments_kernel<__bf16, 1>);
     DTT_CHECK_LAUNCH("unpack_moments_kernel");
   }
   return 1;

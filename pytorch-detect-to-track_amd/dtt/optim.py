@@ -120,8 +120,9 @@ def _stream(dev):
 
 
 # ------------------------------------------------------------------------------------------------ gradient norm
-def _norm_and_factor(grads, max_norm):
-    """(2,) float32: the norm of all gradients (a _List on one GPU) and the factor min(1, max_norm / (norm + 1e-6))."""
+def _norm_and_factor(grads, max_norm, scale=False):
+    """(2,) float32: the norm of all gradients (a _List on one GPU) and the factor min(1, max_norm / (norm + 1e-6)); scale: the
+    gradients are multiplied by it."""
     n = len(grads)
     device = grads.tensors[0].device
     out = torch.empty(2, dtype=torch.float32, device=device)
@@ -129,8 +130,8 @@ def _norm_and_factor(grads, max_norm):
     nbytes = L.dtt_grad_norm_workspace_bytes(n, grads.counts)
     ws = torch.empty(nbytes // 8, dtype=torch.float64, device=device)
     with _on(grads.device):
-        check(L.dtt_grad_norm(n, grads.ptrs, grads.counts, grads.types, max_norm, out.data_ptr(), ws.data_ptr(), nbytes, _stream(grads.device)),
-              "grad_norm")
+        check((L.dtt_grad_clip if scale else L.dtt_grad_norm)(n, grads.ptrs, grads.counts, grads.types, max_norm, out.data_ptr(), ws.data_ptr(),
+                                                              nbytes, _stream(grads.device)), "grad_clip" if scale else "grad_norm")
     return out
 
 
@@ -154,9 +155,7 @@ def clip_grads_(grads, max_norm):
     grads = _gradients("clip_grads_", grads)
     if not len(grads):
         return torch.zeros(())
-    out = _norm_and_factor(grads, max_norm)
-    with _on(grads.device):
-        check(_lib.lib().dtt_grad_scale(len(grads), grads.ptrs, grads.counts, grads.types, out.data_ptr() + 4, _stream(grads.device)), "grad_scale")
+    out = _norm_and_factor(grads, max_norm, scale=True)
     _written(grads.tensors)
     return out[0]
 

@@ -154,8 +154,10 @@ def test_library_refuses_bad_arguments_without_a_gpu():
                     (dict(limit=-1.0), "negative"), (dict(limit=float("nan")), "negative"), (dict(wb=1), "workspace"), (dict(out=None), "null"),
                     (dict(n=N((1 << 34) + 1)), "element count"), (dict(g=None), "null")):
         assert norm(**kw) == 0 and why in _lib.last_error(), (kw, _lib.last_error())
-    assert L.dtt_grad_scale(2, P(base, base + 16), N(8, 8), I(0, 0), base + 1024, None) == 0 and "share memory" in _lib.last_error()
-    assert L.dtt_grad_scale(1, P(base), N(8), I(0), None, None) == 0 and "null" in _lib.last_error()
+    assert L.dtt_grad_clip(2, P(base, base + 16), N(8, 8), I(0, 0), 1.0, base + 1024, ws, 4096, None) == 0 and "share memory" in _lib.last_error()
+    assert L.dtt_grad_clip(1, P(base), N(8), I(0), 1.0, None, ws, 4096, None) == 0 and "null" in _lib.last_error()
+    assert L.dtt_grad_clip(1, P(base), N(8), I(0), -1.0, base + 1024, ws, 4096, None) == 0 and "negative" in _lib.last_error()
+    assert L.dtt_grad_clip(1, P(base), N(8), I(0), 1.0, base + 1024, ws, 0, None) == 0 and "workspace" in _lib.last_error()
 
     def step(p=(base, base + 64), g=(base + 128, base + 192), m=(base + 256, base + 320), v=(base + 384, base + 448), s=(base + 512, base + 516),
              n=(16, 16), dtype=0, lr=(1e-3, 1e-3), wd=(0.0, 0.0), b1=0.9, b2=0.999, eps=1e-8, limit=-1.0, clip=None, skip=0, w=ws, wb=4096):
