@@ -140,12 +140,16 @@ PyObject* differ(PyObject*, PyObject* args) {
   return PyLong_FromLong(-1);
 }
 
-// rows_of(a, b, block, columns) -> -1, or the first i where b[i] is not a contiguous int16 matrix of `columns` columns and a row for
-// every `block` elements of a[i]
+bool rows_for(const at::Tensor& t, const at::Tensor& rows, long block) {
+  return type_code(rows) == kI16 && rows.dim() == 2 && rows.size(0) == (t.numel() + block - 1) / block && rows.size(1) == 2 && rows.is_contiguous();
+}
+
+// rows_of(a, b, block) -> -1, or the first i where b[i] is not a contiguous int16 matrix of two columns and a row for every `block`
+// elements of a[i]
 PyObject* rows_of(PyObject*, PyObject* args) {
   PyObject *a, *b;
-  long block, columns;
-  if (!PyArg_ParseTuple(args, "OOll", &a, &b, &block, &columns) || !is_list(a, "rows_of") || !is_list(b, "rows_of")) return nullptr;
+  long block;
+  if (!PyArg_ParseTuple(args, "OOl", &a, &b, &block) || !is_list(a, "rows_of") || !is_list(b, "rows_of")) return nullptr;
   const Py_ssize_t n = PyList_GET_SIZE(a);
   if (PyList_GET_SIZE(b) != n || block < 1) {
     PyErr_SetString(PyExc_ValueError, "rows_of: lists of different lengths");
@@ -158,9 +162,7 @@ PyObject* rows_of(PyObject*, PyObject* args) {
         PyErr_SetString(PyExc_TypeError, "expected tensors");
         return nullptr;
       }
-      const at::Tensor &x = THPVariable_Unpack(oa), &y = THPVariable_Unpack(ob);
-      if (type_code(y) != kI16 || y.dim() != 2 || y.size(0) != (x.numel() + block - 1) / block || y.size(1) != columns || !y.is_contiguous())
-        return PyLong_FromSsize_t(i);
+      if (!rows_for(THPVariable_Unpack(oa), THPVariable_Unpack(ob), block)) return PyLong_FromSsize_t(i);
     }
   } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
@@ -172,18 +174,100 @@ PyObject* rows_of(PyObject*, PyObject* args) {
   return PyLong_FromLong(-1);
 }
 
-// bump(list): the kernels wrote these tensors behind autograd's back; tell it, as torch's own in-place operations do
-PyObject* bump(PyObject*, PyObject* list) {
-  if (!is_list(list, "bump")) return nullptr;
+// step_lists([params, grads, steps, m, v] or [..., bases], type code of the moments, block) -> None, or (type code, device, tuple of
+// address arrays, element counts): what a step hands to the library where everything is as it has to be -- one type among the parameters,
+// dense, gradients and moments in their shape and order, one device.  None says only that it is not; the caller looks closer.
+PyObject* step_lists(PyObject*, PyObject* args) {
+  PyObject* lists;
+  long moment, block;
+  if (!PyArg_ParseTuple(args, "Oll", &lists, &moment, &block) || !is_list(lists, "step_lists")) return nullptr;
+  const Py_ssize_t k = PyList_GET_SIZE(lists);
+  PyObject* l[6];
+  if (k != 5 && k != 6) {
+    PyErr_SetString(PyExc_ValueError, "step_lists: five or six lists");
+    return nullptr;
+  }
+  for (Py_ssize_t j = 0; j < k; ++j) {
+    l[j] = PyList_GET_ITEM(lists, j);
+    if (!is_list(l[j], "step_lists")) return nullptr;
+    if (PyList_GET_SIZE(l[j]) != PyList_GET_SIZE(l[0])) Py_RETURN_NONE;
+  }
+  const Py_ssize_t n = PyList_GET_SIZE(l[0]);
+  if (n == 0) Py_RETURN_NONE;
+  PyObject* out = PyTuple_New(k);
+  PyObject* counts = PyBytes_FromStringAndSize(nullptr, n * 8);
+  uint64_t* at[6];
+  bool whole = out && counts;
+  for (Py_ssize_t j = 0; whole && j < k; ++j) {
+    PyObject* b = PyBytes_FromStringAndSize(nullptr, n * 8);
+    if (b) {
+      PyTuple_SET_ITEM(out, j, b);
+      at[j] = reinterpret_cast<uint64_t*>(PyBytes_AS_STRING(b));
+    }
+    whole = b != nullptr;
+  }
+  if (!whole) {
+    Py_XDECREF(out); Py_XDECREF(counts);
+    return nullptr;
+  }
+  int64_t* c = reinterpret_cast<int64_t*>(PyBytes_AS_STRING(counts));
+  int type = kOther;
+  long device = kNone;
+  bool plain = true;
   try {
-    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
-      PyObject* o = PyList_GET_ITEM(list, i);
-      if (!THPVariable_Check(o)) {
-        PyErr_SetString(PyExc_TypeError, "expected tensors");
-        return nullptr;
+    for (Py_ssize_t i = 0; plain && i < n; ++i) {
+      const at::Tensor* t[6];
+      for (Py_ssize_t j = 0; plain && j < k; ++j) {
+        PyObject* o = PyList_GET_ITEM(l[j], i);
+        plain = THPVariable_Check(o);
+        if (!plain) break;
+        t[j] = &THPVariable_Unpack(o);
+        plain = t[j]->is_cuda() && (device == kNone || t[j]->get_device() == device);
+        if (plain) device = t[j]->get_device();
       }
-      const at::Tensor& t = THPVariable_Unpack(o);
-      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+      if (!plain) break;
+      const at::Tensor& p = *t[0];
+      if (i == 0) type = type_code(p);
+      plain = type >= kF32 && type <= kF16 && type_code(p) == type && dense(p) && type_code(*t[1]) == type &&
+              type_code(*t[2]) == kF32 && t[2]->numel() == 1 && type_code(*t[3]) == moment && type_code(*t[4]) == moment;
+      for (int j = 1; plain && j < 5; ++j)
+        if (j != 2) plain = t[j]->sizes() == p.sizes() && same_order(p, *t[j]);
+      if (plain && k == 6) plain = rows_for(p, *t[5], block);
+      if (!plain) break;
+      for (Py_ssize_t j = 0; j < k; ++j) at[j][i] = reinterpret_cast<uint64_t>(t[j]->data_ptr());
+      c[i] = p.numel();
+    }
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    Py_DECREF(out); Py_DECREF(counts);
+    return nullptr;
+  } catch (...) {
+    PyErr_SetString(PyExc_RuntimeError, "step_lists: unknown C++ exception");
+    Py_DECREF(out); Py_DECREF(counts);
+    return nullptr;
+  }
+  if (!plain) {
+    Py_DECREF(out); Py_DECREF(counts);
+    Py_RETURN_NONE;
+  }
+  return Py_BuildValue("(ilNN)", type, device, out, counts);
+}
+
+// bump(list, ...): the kernels wrote these tensors behind autograd's back; tell it, as torch's own in-place operations do
+PyObject* bump(PyObject*, PyObject* args) {
+  try {
+    for (Py_ssize_t j = 0; j < PyTuple_GET_SIZE(args); ++j) {
+      PyObject* list = PyTuple_GET_ITEM(args, j);
+      if (!is_list(list, "bump")) return nullptr;
+      for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
+        PyObject* o = PyList_GET_ITEM(list, i);
+        if (!THPVariable_Check(o)) {
+          PyErr_SetString(PyExc_TypeError, "expected tensors");
+          return nullptr;
+        }
+        const at::Tensor& t = THPVariable_Unpack(o);
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+      }
     }
   } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
@@ -198,7 +282,8 @@ PyObject* bump(PyObject*, PyObject* list) {
 PyMethodDef methods[] = {{"describe", describe, METH_O, "addresses, element counts, types, device, common type, first not dense"},
                          {"differ", differ, METH_VARARGS, "first place where two lists differ in shape or memory order"},
                          {"rows_of", rows_of, METH_VARARGS, "first matrix that has not a row for every block of its tensor"},
-                         {"bump", bump, METH_O, "count a version of every tensor"},
+                         {"step_lists", step_lists, METH_VARARGS, "the arrays of an optimizer step, or None"},
+                         {"bump", bump, METH_VARARGS, "count a version of every tensor"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensorlist", "lists of tensors for multi-tensor calls", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -103,8 +103,7 @@ def _limit(what, max_norm):
 
 def _written(*lists):
     """The kernels write behind autograd's back: tell it, as torch's own in-place operations do."""
-    for x in lists:
-        _tensorlist().bump(x)
+    _tensorlist().bump(*lists)
 
 
 _HERE = contextlib.nullcontext()
@@ -191,106 +190,115 @@ def _numbers(what, name, value, n):
     return array("d", [value]) * n
 
 
-class _Step:
-    """The arguments of one step, checked; `launch` sends the tensors of each element type."""
+def _rates(what, lr, n):
+    """(numbers, addresses of those in device memory or None, the tensors among them)"""
+    if isinstance(lr, torch.Tensor):
+        lr = [lr] * n
+    if not isinstance(lr, (list, tuple)) or not any(isinstance(x, torch.Tensor) for x in lr):
+        return _numbers(what, "lr", lr, n), None, []
+    tensors = [x for x in lr if isinstance(x, torch.Tensor)]
+    for x in tensors:
+        if x.numel() != 1 or x.dtype != torch.float32:
+            raise TypeError("%s: a learning rate in device memory is one float32 (got %s, %s)" % (what, tuple(x.shape), x.dtype))
+    return (_numbers(what, "lr", [0.0 if isinstance(x, torch.Tensor) else x for x in lr], n),
+            array("Q", [x.data_ptr() if isinstance(x, torch.Tensor) else 0 for x in lr]), tensors)
 
-    def __init__(self, what, params, grads, moments, types, steps, lr, betas, eps, weight_decay, max_norm, skip_nonfinite, clip):
-        self.what = what
-        lists = [list(x) for x in (params, grads, steps) + tuple(moments)]
-        n = len(lists[0])
-        if any(len(x) != n for x in lists):
-            raise ValueError("%s: the lists differ in length (%s)" % (what, ", ".join(str(len(x)) for x in lists)))
-        self.beta1, self.beta2 = (float(b) for b in betas)
-        self.eps = float(eps)
-        if not (0.0 <= self.beta1 < 1.0 and 0.0 <= self.beta2 < 1.0):
-            raise ValueError("%s: betas must lie in [0, 1) (got %r)" % (what, betas))
-        if not self.eps >= 0.0:
-            raise ValueError("%s: eps must not be negative (got %r)" % (what, eps))
-        max_norm = None if max_norm is None else _limit(what, max_norm)
-        self.skip_nonfinite = bool(skip_nonfinite)
-        if clip is not None and (max_norm is not None or clip.dtype != torch.float32 or tuple(clip.shape) != (2,) or not clip.is_contiguous()):
-            raise ValueError("%s: clip is norm and factor, two float32, and stands in place of max_norm" % what)
-        # rates in device memory stand beside numbers of 0
-        self.rates = None
-        rates = lr if isinstance(lr, (list, tuple)) else [lr]
-        on_device = [x for x in rates if isinstance(x, torch.Tensor)]
-        if on_device:
-            for x in on_device:
-                if x.numel() != 1 or x.dtype != torch.float32:
-                    raise TypeError("%s: a learning rate in device memory is one float32 (got %s, %s)" % (what, tuple(x.shape), x.dtype))
-            rates = list(rates) if isinstance(lr, (list, tuple)) else [lr] * n
-            self.rates = array("Q", [x.data_ptr() if isinstance(x, torch.Tensor) else 0 for x in rates])
-            lr = [0.0 if isinstance(x, torch.Tensor) else x for x in rates]
-        self.lr = _numbers(what, "lr", lr, n)
-        self.decay = _numbers(what, "weight_decay", weight_decay, n)
-        self.n = n
-        if n == 0:
-            return
-        p, g, s = (_List(what, x) for x in lists[:3])
-        p.floats(what, "parameters").dense(what, "parameters")
-        if g.types != p.types:
-            raise TypeError("%s: a gradient has its parameter's type (got %s for %s)" % ((what,) + next(
-                (y.dtype if y.layout == torch.strided else y.layout, x.dtype) for x, y in zip(lists[0], lists[1])
-                if x.dtype != y.dtype or y.layout != torch.strided)))
-        at = _tensorlist().differ(lists[0], lists[1])
-        while at >= 0:
-            x, y = lists[0][at >> 1], lists[1][at >> 1]
-            if at & 1 == 0:
-                raise ValueError("%s: a gradient has its parameter's shape (got %s for %s)" % (what, tuple(y.shape), tuple(x.shape)))
-            # a gradient in another order of its dimensions (or an expanded one) is brought into the parameter's
-            with torch.no_grad():
-                lists[1] = [y if x.shape != y.shape or _same_order(x, y) else torch.empty_like(x).copy_(y) for x, y in zip(lists[0], lists[1])]
-            g = _List(what, lists[1])
-            at = _tensorlist().differ(lists[0], lists[1])
-        if s.type != 0 or s.counts != _ONE * n:
-            bad = next(t for t in lists[2] if t.dtype != torch.float32 or t.numel() != 1 or t.layout != torch.strided)
-            raise TypeError("%s: a step counter is one float32 (got %s, %s)" % (what, tuple(bad.shape), bad.dtype))
-        m = [_List(what, x) for x in lists[3:]]
-        extra = on_device + ([clip] if clip is not None else [])
-        self.dev = _device_of(what, [p, g, s] + m + ([_List(what, extra)] if extra else []))
-        for x, want in zip(m, types):
-            if x.type != want:
-                raise TypeError("%s: moments must be %s (got %s)" % (what, "float32" if want == 0 else "uint8", sorted({str(t.dtype) for t in x.tensors})))
-            at = _tensorlist().differ(lists[0], x.tensors)
-            if at >= 0:
-                t, q = x.tensors[at >> 1], lists[0][at >> 1]
-                raise ValueError("%s: moments have their parameter's shape and memory order (got %s, strides %s for %s, strides %s)" %
-                                 (what, tuple(t.shape), t.stride(), tuple(q.shape), q.stride()))
-        self.max_norm = -1.0
-        if clip is None and (max_norm is not None or self.skip_nonfinite):
-            max_norm = math.inf if max_norm is None else max_norm
-            if p.type >= 0:      # one call: the library computes the norm on its way
-                self.max_norm = max_norm
-                clip = torch.empty(2, dtype=torch.float32, device=lists[0][0].device)
-            else:
-                clip = _norm_and_factor(g, max_norm)
-        self.params, self.grads, self.steps, self.moments, self.clip = p, g, s, m, clip
 
-    def launch(self, call):
-        """call(parts of one element type: lists, lr, device rates, decay, at; tail) for every element type among the parameters.
-        Returns the norm."""
-        if self.n == 0:
-            return None
-        lists = [self.params, self.grads, self.steps] + self.moments
-        groups = [(self.params.type, lists, self.lr, self.rates, self.decay, None)]
-        if self.params.type == -2:
-            groups = []
-            by_type = {}
-            for i, t in enumerate(array("i", self.params.types)):
-                by_type.setdefault(t, []).append(i)
-            for t, at in by_type.items():
-                groups.append((t, [_List(self.what, [x.tensors[i] for i in at]) for x in lists], array("d", [self.lr[i] for i in at]),
-                               None if self.rates is None else array("Q", [self.rates[i] for i in at]), array("d", [self.decay[i] for i in at]), at))
-        L = _lib.lib()
-        device = self.params.tensors[0].device
-        with _on(self.dev):
-            for dtype, parts, lr, rates, decay, at in groups:
-                nbytes = L.dtt_adamw_workspace_bytes(len(parts[0]), parts[0].counts)
-                ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-                call(L, len(parts[0]), dtype, [x.ptrs for x in parts], parts[0].counts, lr.tobytes(), None if rates is None else rates.tobytes(),
-                     decay.tobytes(), at, (self.max_norm, None if self.clip is None else self.clip.data_ptr(), int(self.skip_nonfinite), ws.data_ptr(), nbytes, _stream(self.dev)))
-        _written(*[x.tensors for x in [self.params, self.steps] + self.moments])
-        return None if self.clip is None else self.clip[0]
+def _mend(what, lists, moment_type):
+    """Why the lists of a step are not plain: raises what is wrong with them, or returns them with gradients in their parameters' order."""
+    params, grads, steps = lists[:3]
+    p, g, s = (_List(what, x) for x in lists[:3])
+    p.floats(what, "parameters").dense(what, "parameters")
+    if g.types != p.types:
+        raise TypeError("%s: a gradient has its parameter's type (got %s for %s)" % ((what,) + next(
+            (y.dtype if y.layout == torch.strided else y.layout, x.dtype) for x, y in zip(params, grads) if x.dtype != y.dtype or y.layout != torch.strided)))
+    for x, y in zip(params, grads):
+        if x.shape != y.shape:
+            raise ValueError("%s: a gradient has its parameter's shape (got %s for %s)" % (what, tuple(y.shape), tuple(x.shape)))
+    if s.type != 0 or s.counts != _ONE * len(steps):
+        bad = next(t for t in steps if t.dtype != torch.float32 or t.numel() != 1 or t.layout != torch.strided)
+        raise TypeError("%s: a step counter is one float32 (got %s, %s)" % (what, tuple(bad.shape), bad.dtype))
+    _device_of(what, [p, g, s] + [_List(what, x) for x in lists[3:]])
+    for x in lists[3:5]:
+        m = _List(what, x)
+        if m.type != moment_type:
+            raise TypeError("%s: moments must be %s (got %s)" % (what, "float32" if moment_type == 0 else "uint8", sorted({str(t.dtype) for t in x})))
+        at = _tensorlist().differ(params, x)
+        if at >= 0:
+            t, q = x[at >> 1], params[at >> 1]
+            raise ValueError("%s: moments have their parameter's shape and memory order (got %s, strides %s for %s, strides %s)" %
+                             (what, tuple(t.shape), t.stride(), tuple(q.shape), q.stride()))
+    if len(lists) == 6:
+        _check_bases(what, params, lists[5])
+    # a gradient in another order of its dimensions (or an expanded one) is brought into the parameter's
+    with torch.no_grad():
+        grads = [y if _same_order(x, y) else torch.empty_like(x).copy_(y) for x, y in zip(params, grads)]
+    return [params, grads] + lists[2:]
+
+
+def _step(what, lists, moment_type, lr, betas, eps, weight_decay, max_norm, skip_nonfinite, clip, seed=0, ids=None):
+    """One step of the lists [params, grads, steps, m, v] (32-bit moments) or [..., bases] (8-bit); returns the norm or None."""
+    lists = [x if type(x) is list else list(x) for x in lists]
+    n = len(lists[0])
+    if any(len(x) != n for x in lists) or (ids is not None and len(ids) != n):
+        raise ValueError("%s: the lists differ in length (%s)" % (what, ", ".join(str(len(x)) for x in lists + ([] if ids is None else [ids]))))
+    beta1, beta2 = betas
+    if not (0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0):
+        raise ValueError("%s: betas must lie in [0, 1) (got %r)" % (what, betas))
+    if not eps >= 0.0:
+        raise ValueError("%s: eps must not be negative (got %r)" % (what, eps))
+    if max_norm is not None:
+        max_norm = _limit(what, max_norm)
+    if clip is not None and (max_norm is not None or clip.dtype != torch.float32 or tuple(clip.shape) != (2,) or not clip.is_contiguous()):
+        raise ValueError("%s: clip is norm and factor, two float32, and stands in place of max_norm" % what)
+    rates, device_rates, extra = _rates(what, lr, n)
+    decay = _numbers(what, "weight_decay", weight_decay, n)
+    if n == 0:
+        return None
+    T = _tensorlist()
+    plain = T.step_lists(lists, moment_type, BLOCK)
+    if plain is None:
+        lists = _mend(what, lists, moment_type)
+        by_type = {}
+        for i, p in enumerate(lists[0]):
+            by_type.setdefault(p.dtype, []).append(i)
+        if len(by_type) > 1:     # one norm over all of them, one call for each type
+            if clip is None and (max_norm is not None or skip_nonfinite):
+                clip = _norm_and_factor(_List(what, lists[1]), math.inf if max_norm is None else max_norm)
+            rates = lr if isinstance(lr, (list, tuple)) else [lr] * n
+            for at in by_type.values():
+                _step(what, [[x[i] for i in at] for x in lists], moment_type, [rates[i] for i in at], betas, eps, [decay[i] for i in at], None,
+                      skip_nonfinite, clip, seed, at if ids is None else [ids[i] for i in at])
+            return None if clip is None else clip[0]
+        plain = T.step_lists(lists, moment_type, BLOCK)
+        if plain is None:
+            raise RuntimeError("%s: the lists changed while they were read" % what)
+    dtype, dev, ptrs, counts = plain
+    if extra or clip is not None:
+        for x in extra + ([] if clip is None else [clip]):
+            if x.get_device() != dev:
+                raise ValueError("%s: all tensors must be on one device (got cuda:%d and %s)" % (what, dev, x.device))
+    L = _lib.lib()
+    device = lists[0][0].device
+    limit = -1.0
+    if clip is None and (max_norm is not None or skip_nonfinite):    # the library computes the norm on its way
+        limit = math.inf if max_norm is None else max_norm
+        clip = torch.empty(2, dtype=torch.float32, device=device)
+    nbytes = L.dtt_adamw_workspace_bytes(n, counts)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    rates, decay = rates.tobytes(), decay.tobytes()
+    device_rates = None if device_rates is None else device_rates.tobytes()
+    tail = (beta1, beta2, eps, limit, None if clip is None else clip.data_ptr(), 1 if skip_nonfinite else 0, ws.data_ptr(), nbytes, _stream(dev))
+    with _on(dev):
+        if moment_type == 0:
+            p, g, s, m, v = ptrs
+            check(L.dtt_adamw_step(n, dtype, p, g, m, v, counts, s, rates, device_rates, decay, *tail), what)
+        else:
+            p, g, s, m, v, b = ptrs
+            ids = None if ids is None else array("I", [int(i) & 0xFFFFFFFF for i in ids]).tobytes()
+            check(L.dtt_adamw8_step(n, dtype, p, g, m, v, b, counts, s, rates, device_rates, decay, ids, int(seed) & 0xFFFFFFFF, *tail), what)
+    T.bump(lists[0], *lists[2:])
+    return None if clip is None else clip[0]
 
 
 def adamw_(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None,
@@ -304,12 +312,7 @@ def adamw_(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999
     max_norm: c = min(1, max_norm / (norm + 1e-6)) of the norm over all gradients (which stay as they are), else c = 1.
     skip_nonfinite: where that norm is infinite or NaN, nothing changes, the counters neither.  clip: norm and factor computed before
     (float32, 2 entries), in place of max_norm.  Returns the norm (float32 scalar on the device), or None without any of the three."""
-    s = _Step("adamw_", params, grads, (exp_avgs, exp_avg_sqs), (0, 0), steps, lr, betas, eps, weight_decay, max_norm, skip_nonfinite, clip)
-
-    def call(L, n, dtype, ptrs, numel, rates, rates_device, decay, at, tail):
-        p, g, counters, m, v = ptrs
-        check(L.dtt_adamw_step(n, dtype, p, g, m, v, numel, counters, rates, rates_device, decay, s.beta1, s.beta2, s.eps, *tail), "adamw_")
-    return s.launch(call)
+    return _step("adamw_", [params, grads, steps, exp_avgs, exp_avg_sqs], 0, lr, betas, eps, weight_decay, max_norm, skip_nonfinite, clip)
 
 
 def blocks_of(numel):
@@ -325,38 +328,16 @@ def adamw8_(params, grads, exp_avgs, exp_avg_sqs, bases, steps, *, lr, betas=(0.
     2^-15.7 below its block's largest is not moved.  The rounding of a moment is dithered, right on average, by a hash of seed, ids
     (default: the position in the list), step counter and element; the same inputs give the same codes.  Infinite and NaN moments stay
     in their element, as NaN."""
-    bases = list(bases)
-    s = _Step("adamw8_", params, grads, (exp_avgs, exp_avg_sqs), (_UINT8, _UINT8), steps, lr, betas, eps, weight_decay, max_norm, skip_nonfinite,
-              clip)
-    ids = None if ids is None else [int(i) & 0xFFFFFFFF for i in ids]
-    if len(bases) != s.n or (ids is not None and len(ids) != s.n):
-        raise ValueError("adamw8_: %d bases and %s ids for %d tensors" % (len(bases), "no" if ids is None else len(ids), s.n))
-    if s.n == 0:
-        return None
-    described = _List("adamw8_", bases)
-    _check_bases("adamw8_", s.params, described, s.dev)
-
-    def call(L, n, dtype, ptrs, numel, rates, rates_device, decay, at, tail):
-        p, g, counters, m, v = ptrs
-        where, names = described.ptrs, ids
-        if at is not None:
-            where, names = _List("adamw8_", [bases[i] for i in at]).ptrs, at if ids is None else [ids[i] for i in at]
-        check(L.dtt_adamw8_step(n, dtype, p, g, m, v, where, numel, counters, rates, rates_device, decay,
-                                None if names is None else array("I", names).tobytes(), int(seed) & 0xFFFFFFFF, s.beta1, s.beta2, s.eps, *tail),
-              "adamw8_")
-    norm = s.launch(call)
-    _written(bases)
-    return norm
+    return _step("adamw8_", [params, grads, steps, exp_avgs, exp_avg_sqs, bases], _UINT8, lr, betas, eps, weight_decay, max_norm, skip_nonfinite,
+                 clip, seed, ids)
 
 
-def _check_bases(what, like, bases, dev):
-    at = _tensorlist().rows_of(like.tensors, bases.tensors, BLOCK, 2)
+def _check_bases(what, like, bases):
+    at = _tensorlist().rows_of(like, bases, BLOCK)
     if at >= 0:
-        b = bases.tensors[at]
+        b = bases[at]
         raise ValueError("%s: bases are int16, contiguous, (blocks_of(numel), 2): two for each %d elements (got %s, %s, strides %s for %d elements)" %
-                         (what, BLOCK, b.dtype, tuple(b.shape), b.stride(), like.tensors[at].numel()))
-    if _device_of(what, [bases]) != dev:
-        raise ValueError("%s: all tensors must be on one device" % what)
+                         (what, BLOCK, b.dtype, tuple(b.shape), b.stride(), like[at].numel()))
 
 
 def unpack_moments_(exp_avgs, exp_avg_sqs, bases, out_avgs, out_avg_sqs):
@@ -377,8 +358,8 @@ def unpack_moments_(exp_avgs, exp_avg_sqs, bases, out_avgs, out_avg_sqs):
     m.dense(what, "codes")
     if any(_tensorlist().differ(lists[0], t) >= 0 for t in (lists[1], lists[3], lists[4])):
         raise ValueError("%s: codes and values have one shape and memory order" % what)
-    dev = _device_of(what, [m, v, x, y])
-    _check_bases(what, m, b, dev)
+    dev = _device_of(what, [m, v, b, x, y])
+    _check_bases(what, lists[0], lists[2])
     with _on(dev):
         check(_lib.lib().dtt_adamw8_unpack(n, m.ptrs, v.ptrs, b.ptrs, m.counts, x.type, x.ptrs, y.ptrs, _stream(dev)), what)
     _written(lists[3], lists[4])

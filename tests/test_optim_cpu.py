@@ -115,7 +115,7 @@ def test_refusals_before_any_gpu_work():
         O.adamw_([torch.zeros(10, 3)[::2]] * 2, g, m, v, s, lr=1e-3)
     with pytest.raises(TypeError):
         O.adamw_(p, [None, g[1]], m, v, s, lr=1e-3)
-    with pytest.raises(ValueError, match="ids"):
+    with pytest.raises(ValueError, match="differ in length"):
         O.adamw8_([], [], [], [], [], [], lr=1e-3, ids=[1])
     with pytest.raises(ValueError, match="clip"):
         O.adamw_(p, g, m, v, s, lr=1e-3, clip=torch.zeros(3))
