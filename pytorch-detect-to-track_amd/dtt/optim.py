@@ -297,7 +297,7 @@ def _step(what, lists, moment_type, lr, betas, eps, weight_decay, max_norm, skip
             p, g, s, m, v, b = ptrs
             ids = None if ids is None else array("I", [int(i) & 0xFFFFFFFF for i in ids]).tobytes()
             check(L.dtt_adamw8_step(n, dtype, p, g, m, v, b, counts, s, rates, device_rates, decay, ids, int(seed) & 0xFFFFFFFF, *tail), what)
-    T.bump(lists[0], *lists[2:])
+    T.bump(lists[0])
     return None if clip is None else clip[0]
 
 
@@ -504,46 +504,55 @@ class GroupedAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        work, fresh, grads = {}, [], []
-        place = -1
+        work, fresh = {}, []
+        state, place = self.state, -1
+        names = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("exp_avg_code", "exp_avg_sq_code")
         for g in self.param_groups:
+            key = (g["betas"], g["eps"])
+            key = key if type(key[0]) is tuple else (tuple(key[0]), key[1])
+            rows = work.get(key)
+            if rows is None:
+                rows = work[key] = ([], [], [], [], [])
+            lr, decay = g["lr"], g["weight_decay"]
             for p in g["params"]:
                 place += 1
                 grad = p.grad
                 if grad is None:
                     continue
-                if grad.layout != torch.strided:
-                    raise TypeError("GroupedAdamW: gradients must be dense tensors (got %s)" % grad.layout)
-                if p not in self.state or not self.state[p]:
+                if not state.get(p):
                     fresh.append(p)
-                grads.append(grad)
-                work.setdefault((tuple(g["betas"]), g["eps"]), []).append((p, grad, g["lr"], g["weight_decay"], place))
-        if not grads:
+                rows[0].append(p)
+                rows[1].append(grad)
+                rows[2].append(lr)
+                rows[3].append(decay)
+                rows[4].append(place)
+        work = {k: rows for k, rows in work.items() if rows[0]}
+        if not work:
             return loss
-        _device_of("GroupedAdamW", [_List("GroupedAdamW", grads)])
-        if fresh:
+        what = "GroupedAdamW"
+        if fresh:       # (everything that would refuse the step does so before state is made)
+            for rows in work.values():
+                p, g = _List(what, rows[0]).floats(what, "parameters").dense(what, "parameters"), _List(what, rows[1]).floats(what, "gradients")
+                _device_of(what, [p, g])
             self._make_state(fresh)
-        clip = None
-        if self.max_norm is not None or self.skip_nonfinite:
-            checked = _List("GroupedAdamW", grads).floats("GroupedAdamW", "gradients")
-            if checked.odd >= 0:
-                checked = _List("GroupedAdamW", [g if _dense(g) else g.contiguous() for g in grads])
-            clip = _norm_and_factor(checked, math.inf if self.max_norm is None else self.max_norm)
-            self.grad_norm = clip[0]
-        for (betas, eps), rows in work.items():
-            states = []
-            for p, _, _, _, _ in rows:
-                st = self.state[p]
-                first = st["exp_avg"] if self.state_bits == 32 else st["exp_avg_code"]
-                if not _same_order(p, first):   # the parameter took another memory order since (channels-last filters)
-                    self._keep_moments(p, st, *self._moments(p, st))
-                states.append(st)
-            common = dict(lr=[r[2] for r in rows], betas=betas, eps=eps, weight_decay=[r[3] for r in rows], skip_nonfinite=self.skip_nonfinite,
-                          clip=clip)
-            params, gs, counters = [r[0] for r in rows], [r[1] for r in rows], [st["step"] for st in states]
-            if self.state_bits == 32:
-                adamw_(params, gs, [st["exp_avg"] for st in states], [st["exp_avg_sq"] for st in states], counters, **common)
-            else:
-                adamw8_(params, gs, [st["exp_avg_code"] for st in states], [st["exp_avg_sq_code"] for st in states],
-                        [st["block_base"] for st in states], counters, seed=self.seed, ids=[r[4] for r in rows], **common)
+        limit, clip = self.max_norm, None
+        if (limit is not None or self.skip_nonfinite) and len(work) > 1:     # one norm over all of them
+            grads = _List(what, [g if _dense(g) else g.contiguous() for rows in work.values() for g in rows[1]]).floats(what, "gradients")
+            _device_of(what, [grads])
+            clip, limit = _norm_and_factor(grads, math.inf if limit is None else limit), None
+        norm = None
+        for (betas, eps), (params, grads, lr, decay, places) in work.items():
+            states = [state[p] for p in params]
+            m = [st[names[0]] for st in states]
+            at = _tensorlist().differ(params, m)
+            while at >= 0:      # the parameter took another memory order since (channels-last filters)
+                i = at >> 1
+                self._keep_moments(params[i], states[i], *self._moments(params[i], states[i]))
+                m[i] = states[i][names[0]]
+                at = _tensorlist().differ(params, m)
+            lists = [params, grads, [st["step"] for st in states], m, [st[names[1]] for st in states]]
+            if self.state_bits == 8:
+                lists.append([st["block_base"] for st in states])
+            norm = _step(what, lists, 0 if self.state_bits == 32 else _UINT8, lr, betas, eps, decay, limit, self.skip_nonfinite, clip, self.seed, places)
+        self.grad_norm = norm
         return loss
