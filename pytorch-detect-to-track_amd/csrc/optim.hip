@@ -21,7 +21,8 @@ constexpr int kMaxStep8 = 72;     // 6 * 8 + 4
 constexpr int kMaxPrepare = 280;  // 8 + 4 + 1, and kMaxRates different rates
 constexpr int kMaxRates = 8;
 constexpr int kNormWorkgroups = 2048;   // 8 on a CU: all resident at once
-constexpr long kMaxNumel = 1L << 34;   // element / 8 fits the 32-bit hash input; a launch's workgroups (kMaxNumel / 1024 * kMax*) fit an int
+constexpr long kMaxNumel = 1L << 33;   // element / 8 fits the 32-bit hash input, a tensor's workgroups one launch
+constexpr long kMaxWorkgroups = (1L << 24) - 1;   // a launch holds less than 2^32 work-items
 
 enum { kF32 = 0, kBf16 = 1, kF16 = 2 };
 
@@ -623,6 +624,18 @@ struct Spans {
   }
 };
 
+// how many of the next tensors go into one launch: `most` at most, and fewer where their workgroups (of 1024 elements or more) would be
+// more than a launch may have
+int fit(int n, int most, const long* numel) {
+  long workgroups = 0;
+  int k = 0;
+  for (; k < n && k < most; ++k) {
+    workgroups += numel[k] / 1024 + 2;
+    if (k > 0 && workgroups > kMaxWorkgroups) break;
+  }
+  return k;
+}
+
 bool aligned_to(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
 
 long norm_chunk(int n, const long* numel) {
@@ -853,8 +866,8 @@ extern "C" int dtt_adamw_step(int n, int dtype, void* const* params, const void*
   if (!prepare(n, dtype, grads, numel, steps, lr, lr_device, weight_decay, nullptr, 0u, beta1, beta2, max_norm, clip, skip_nonfinite, factors,
                stream)) return 0;
   StepTable tab;
-  for (int i0 = 0; i0 < n; i0 += kMaxStep) {
-    tab.n = n - i0 < kMaxStep ? n - i0 : kMaxStep;
+  for (int i0 = 0; i0 < n; i0 += tab.n) {
+    tab.n = fit(n - i0, kMaxStep, numel + i0);
     int blocks = 0;
     for (int j = 0; j < tab.n; ++j) {
       const int i = i0 + j;
@@ -899,8 +912,8 @@ extern "C" int dtt_adamw8_step(int n, int dtype, void* const* params, const void
   if (!prepare(n, dtype, grads, numel, steps, lr, lr_device, weight_decay, ids, seed, beta1, beta2, max_norm, clip, skip_nonfinite, factors,
                stream)) return 0;
   Step8Table tab;
-  for (int i0 = 0; i0 < n; i0 += kMaxStep8) {
-    tab.n = n - i0 < kMaxStep8 ? n - i0 : kMaxStep8;
+  for (int i0 = 0; i0 < n; i0 += tab.n) {
+    tab.n = fit(n - i0, kMaxStep8, numel + i0);
     const bool four = four_blocks(tab.n, numel + i0);
     int blocks = 0;
     for (int j = 0; j < tab.n; ++j) {
@@ -944,8 +957,8 @@ extern "C" int dtt_adamw8_unpack(int n, const unsigned char* const* exp_avgs, co
   for (int i = 0; i < n; ++i) spans.add(out_avg_sqs[i], numel[i] * es, true);
   DTT_REQUIRE(!spans.clash(), "adamw8_unpack: two of the tensors share memory");
   UnpackTable tab;
-  for (int i0 = 0; i0 < n; i0 += kMaxStep8) {
-    tab.n = n - i0 < kMaxStep8 ? n - i0 : kMaxStep8;
+  for (int i0 = 0; i0 < n; i0 += tab.n) {
+    tab.n = fit(n - i0, kMaxStep8, numel + i0);
     const bool four = four_blocks(tab.n, numel + i0);
     int blocks = 0;
     for (int j = 0; j < tab.n; ++j) {

@@ -149,7 +149,8 @@ def grad_norm(grads):
 
 def clip_grads_(grads, max_norm):
     """Scale all gradients in place by min(1, max_norm / (norm + 1e-6)) and return their norm before that (float32 scalar on their
-    device).  Gradients within the limit are not written.  Mixed float32 / bfloat16 / float16 tensors are one vector."""
+    device).  Gradients within the limit are not written.  Mixed float32 / bfloat16 / float16 tensors are one vector.  An infinite norm
+    gives the factor 0 and NaN gives NaN, as the formula has it; no tensor may appear twice."""
     max_norm = _limit("clip_grads_", max_norm)
     grads = _gradients("clip_grads_", grads)
     if not len(grads):
@@ -547,6 +548,10 @@ class GroupedAdamW(torch.optim.Optimizer):
             at = _tensorlist().differ(params, m)
             while at >= 0:      # the parameter took another memory order since (channels-last filters)
                 i = at >> 1
+                if at & 1 == 0:
+                    raise ValueError("GroupedAdamW: the state of a parameter of shape %s has shape %s" % (tuple(params[i].shape), tuple(m[i].shape)))
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("GroupedAdamW: run a step before capturing one (the state follows a parameter's new memory order)")
                 self._keep_moments(params[i], states[i], *self._moments(params[i], states[i]))
                 m[i] = states[i][names[0]]
                 at = _tensorlist().differ(params, m)

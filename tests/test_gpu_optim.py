@@ -465,6 +465,76 @@ def test_steps_on_another_stream_and_two_at_once():
         assert all(torch.equal(a, b) for x, y in zip(got, w) for a, b in zip(x, y))
 
 
+def test_more_rates_than_a_launch_holds_and_rates_in_device_memory():
+    from dtt.optim import adamw8_, adamw_, blocks_of
+    rs = np.random.RandomState(9)
+    n = 290
+    params = [torch.from_numpy(rs.randn(37).astype(np.float32)).to(DEV) for _ in range(n)]
+    grads = [torch.randn(37, device=DEV) for _ in range(n)]
+    ms, vs = ([torch.zeros(37, device=DEV) for _ in range(n)] for _ in range(2))
+    steps = list(torch.zeros(n, device=DEV).unbind())
+    on_device = [torch.full((1,) if i % 2 else (), 1e-2 / (i + 1), device=DEV) for i in range(n)]
+    lr = [on_device[i] if i % 3 == 0 else 1e-2 / (i + 1) for i in range(n)]
+    decay = [0.1 * (i % 11) for i in range(n)]
+    old = [[f64(x) for x in row] for row in zip(params, grads, ms, vs)]
+    q = [p.clone() for p in params]
+    adamw_(params, grads, ms, vs, steps, lr=lr, weight_decay=decay)
+    codes = [[torch.zeros(37, dtype=torch.uint8, device=DEV) for _ in range(n)] for _ in range(2)]
+    bases = [torch.zeros(blocks_of(37), 2, dtype=torch.int16, device=DEV) for _ in range(n)]
+    adamw8_(q, grads, codes[0], codes[1], bases, list(torch.zeros(n, device=DEV).unbind()), lr=lr, weight_decay=decay)
+    for i, o in enumerate(old):
+        rate = float(on_device[i]) if i % 3 == 0 else lr[i]
+        check_step(*o, 1, params[i], ms[i], vs[i], torch.float32, lr=rate, beta1=0.9, beta2=0.999, eps=1e-8, decay=decay[i])
+        wp, _, _, ep, _, _ = oo.adamw(*o, 1, rate, 0.9, 0.999, 1e-8, decay[i])
+        assert (np.abs(f64(q[i]) - wp) <= ep).all()
+    with pytest.raises(ValueError, match="one device"):
+        adamw_(params, grads, ms, vs, steps, lr=torch.zeros(()))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_tiny_eps_and_subnormal_second_moments(bits):
+    """Gradients whose second moments are subnormal in fp32, beside an eps that does not hide them (the 8-bit step's quotient takes
+    its exact form there)."""
+    from dtt.optim import adamw8_, adamw_, blocks_of
+    n = 512
+    g = torch.from_numpy((np.random.RandomState(2).uniform(3e-21, 3e-19, n) * np.where(np.arange(n) % 2, 1, -1)).astype(np.float32)).to(DEV)
+    for eps in (0.0, 1e-25, 1e-12):
+        p, s = torch.ones(n, device=DEV), torch.zeros((), device=DEV)
+        if bits == 32:
+            adamw_([p], [g], [torch.zeros(n, device=DEV)], [torch.zeros(n, device=DEV)], [s], lr=0.1, betas=(0.5, 0.5), eps=eps, weight_decay=0.0)
+        else:
+            adamw8_([p], [g], [torch.zeros(n, dtype=torch.uint8, device=DEV)], [torch.zeros(n, dtype=torch.uint8, device=DEV)],
+                    [torch.zeros(blocks_of(n), 2, dtype=torch.int16, device=DEV)], [s], lr=0.1, betas=(0.5, 0.5), eps=eps, weight_decay=0.0)
+        x = g.double().cpu().numpy()
+        v = 0.5 * x * x
+        den = np.sqrt(v) / np.sqrt(0.5) + eps
+        # v is rounded to multiples of 2^-149: relative error 2^-149 / v (square and sum), half of it in the root
+        want, rel = 1 - 0.1 / 0.5 * 0.5 * x / den, np.minimum(1.0, 2 * 2.0 ** -149 / v) + 16 * oo.U
+        assert (np.abs(f64(p) - want) <= 0.1 * np.abs(x / den) * rel + 2 * oo.U).all(), (eps, np.abs(f64(p) - want).max())
+
+
+def test_gradients_in_flat_buckets_give_the_same_step():
+    """The data-parallel wrapper hands gradients over as views of flat buckets, none of them aligned: bit for bit the same update."""
+    from dtt.dist import DataParallelSnippets
+    from dtt.optim import GroupedAdamW
+    a, b = _model(6), _model(6)
+    runner = DataParallelSnippets(b, 1, bucket_bytes=4096, force_buckets=True)
+    oa, ob = (GroupedAdamW(m.parameters(), lr=1e-2, max_norm=0.05) for m in (a, b))
+    for t in range(3):
+        torch.manual_seed(t)
+        x = torch.randn(4, 3, 6, 6, device=DEV)
+        oa.zero_grad(set_to_none=True)
+        runner.zero_grad(set_to_none=True)
+        a(x).square().mean().backward()
+        runner(x).square().mean().backward()
+        runner.finish_gradients()
+        for p, q in zip(a.parameters(), b.parameters()):
+            q.grad.copy_(p.grad)             # (the library's convolution gradients need not be the same bits twice)
+        oa.step(); ob.step()
+        # (sums and elements go by index, not by address)
+        assert all(torch.equal(p, q) for p, q in zip(a.parameters(), b.parameters()))
+
+
 def test_offsets_beyond_32_bits():
     """A tensor of more than 2^32 elements (bf16, 8-bit moments): its end is what a small tensor with the same values gives."""
     from dtt.optim import adamw8_, blocks_of, grad_norm
