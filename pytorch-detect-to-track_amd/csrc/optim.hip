@@ -10,6 +10,7 @@
 #include <math.h>
 #include <stdlib.h>
 #include <algorithm>
+#include <type_traits>
 #include "common.h"
 
 namespace {
@@ -28,16 +29,16 @@ enum { kF32 = 0, kBf16 = 1, kF16 = 2 };
 
 // ------------------------------------------------------------------------------------------------ element types
 // Vector accesses at ELEMENT alignment: views of a flat bucket start anywhere, and the memory pipe takes wide accesses at any
-// element boundary (a line that is cut costs a second request, nothing else).  All of them are non-temporal: every byte of a step is
-// used once, and lines that are not kept leave the memory-side cache to the gradients that the norm has just read (Res-101's clipped
-// step 350 -> 316 us, the norm of 1.2 G bf16 422 -> 380 us = 6.4 TB/s).
+// element boundary (a line that is cut costs a second request, nothing else).  They are non-temporal: every byte of a step is used once,
+// and lines that are not kept leave the memory-side cache to the gradients that the norm has just read (Res-101's clipped step 350 -> 316
+// us).  Those alone are kept (KEEP) where there is something left of them when the next launch reads them: see kKeepBytes.
 template <typename T, int N> struct Wide {
   typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
 };
 
-template <typename T, int N> __device__ __forceinline__ void load_f32(const T* p, float (&x)[N]) {
+template <typename T, int N, bool KEEP = false> __device__ __forceinline__ void load_f32(const T* p, float (&x)[N]) {
   typedef typename Wide<T, N>::type V;
-  const V v = __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+  const V v = KEEP ? *reinterpret_cast<const V*>(p) : __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = (float)v[i];
 }
@@ -64,16 +65,20 @@ __device__ __forceinline__ int owner(const int* block0, int n, int b) {
 // ------------------------------------------------------------------------------------------------ gradient norm
 // norm = sqrt(sum of all g^2) and the factor min(1, max_norm / (norm + 1e-6)).  Squares and sums in 64 bits: no overflow for any
 // fp32 gradient, and the order of the partial sums (fixed: chunks, then workgroups in index order) does not show in 32 bits.
+// Gradients of up to kKeepBytes in all are read into the caches, for the launch that reads them again; larger ones pass by.  Clipping of
+// fp32 (us, kept / passing by): 96 MB 49 / 54, 192 MB 93 / 105, 383 MB 194 / 211, 768 MB 404 / 415, 1151 MB 617 / 623; the norm alone of 2.4 GB
+// 422 / 380 (6.4 TB/s).  Res-101's clipped step: 272 / 297.
+constexpr long kKeepBytes = 1L << 30;
 struct NormTable {
   const void* g[kMaxNorm];
   long numel[kMaxNorm];
   int block0[kMaxNorm];
   int dtype[kMaxNorm];
   long chunk;          // elements per workgroup, a multiple of kThreads * 8
-  int n;
+  int n, keep;
 };
 
-template <typename T, int N> __device__ __forceinline__ double square_sum(const T* g, long e0, long e1) {
+template <typename T, int N, bool KEEP> __device__ __forceinline__ double square_sum(const T* g, long e0, long e1) {
   constexpr int kFly = 4;   // vectors on their way per thread
   double acc[N];
 #pragma unroll
@@ -82,7 +87,7 @@ template <typename T, int N> __device__ __forceinline__ double square_sum(const 
   for (; e + (kFly - 1) * kThreads * N + N <= e1; e += kFly * kThreads * N) {
     float x[kFly][N];
 #pragma unroll
-    for (int u = 0; u < kFly; ++u) load_f32<T, N>(g + e + u * kThreads * N, x[u]);
+    for (int u = 0; u < kFly; ++u) load_f32<T, N, KEEP>(g + e + u * kThreads * N, x[u]);
 #pragma unroll
     for (int u = 0; u < kFly; ++u)
 #pragma unroll
@@ -90,7 +95,7 @@ template <typename T, int N> __device__ __forceinline__ double square_sum(const 
   }
   for (; e + N <= e1; e += kThreads * N) {
     float x[N];
-    load_f32<T, N>(g + e, x);
+    load_f32<T, N, KEEP>(g + e, x);
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = __builtin_fma((double)x[i], (double)x[i], acc[i]);
   }
@@ -121,10 +126,13 @@ __global__ __launch_bounds__(kThreads) void grad_norm_kernel(NormTable tab, doub
   const int i = owner(tab.block0, tab.n, blockIdx.x);
   const long e0 = (long)((int)blockIdx.x - tab.block0[i]) * tab.chunk;
   const long e1 = e0 + tab.chunk < tab.numel[i] ? e0 + tab.chunk : tab.numel[i];
-  double s;
-  if (tab.dtype[i] == kF32) s = square_sum<float, 4>(static_cast<const float*>(tab.g[i]), e0, e1);
-  else if (tab.dtype[i] == kBf16) s = square_sum<__bf16, 8>(static_cast<const __bf16*>(tab.g[i]), e0, e1);
-  else s = square_sum<_Float16, 8>(static_cast<const _Float16*>(tab.g[i]), e0, e1);
+  const auto sum = [&](auto keep) {
+    constexpr bool KEEP = decltype(keep)::value;
+    if (tab.dtype[i] == kF32) return square_sum<float, 4, KEEP>(static_cast<const float*>(tab.g[i]), e0, e1);
+    if (tab.dtype[i] == kBf16) return square_sum<__bf16, 8, KEEP>(static_cast<const __bf16*>(tab.g[i]), e0, e1);
+    return square_sum<_Float16, 8, KEEP>(static_cast<const _Float16*>(tab.g[i]), e0, e1);
+  };
+  double s = tab.keep ? sum(std::true_type{}) : sum(std::false_type{});
   s = workgroup_sum<kThreads / 64>(s);
   if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
@@ -672,7 +680,10 @@ namespace {
 int norm_partials(int n, const void* const* grads, const long* numel, const int* dtypes, int dtype, double* partial, hipStream_t stream) {
   const long chunk = n > 0 ? norm_chunk(n, numel) : 1;
   int blocks = 0;
+  long bytes = 0;
+  for (int i = 0; i < n; ++i) bytes += numel[i] * type_bytes(dtypes ? dtypes[i] : dtype);
   NormTable tab;
+  tab.keep = bytes <= kKeepBytes;
   for (int i = 0; i < n;) {
     tab.n = 0; tab.chunk = chunk;
     int here = 0;
