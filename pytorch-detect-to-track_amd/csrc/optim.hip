@@ -6,7 +6,6 @@
 // A tensor is a dense run of memory in whatever order its dimensions lie; a workgroup owns one chunk of one tensor and finds it
 // from the prefix sums of the tensors' workgroup counts.  All kernels stream: they are bound by HBM, so what they are measured
 // against is bytes / bandwidth.
-#include <float.h>
 #include <math.h>
 #include <stdlib.h>
 #include <algorithm>
@@ -273,25 +272,16 @@ struct Consts {
   float beta1, one_beta1, beta2, one_beta2, eps;
 };
 
-// The quotient of the update for 8-bit moments, whose kernel has about as many instructions as it has bytes: v_sqrt and v_rcp, each good
-// to 2^-24, in place of the exactly rounded sequences (302 M bf16: step and unpacking 985 -> 884 us).  v_sqrt takes a v below 2^-126 for 0:
-// beside eps >= 2^-32 that is below 2^-24 of the denominator (root is at most 2^7 for beta2 <= 0.9999); a smaller eps takes the exact
-// sequences (a uniform branch).
-__device__ __forceinline__ float quotient8(float m, float v, float root, float eps) {
-  if (eps < 0x1p-32f) return m / (sqrtf(v) * root + eps);
-  return m * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v) * root + eps);
-}
-
 // m <- beta1 m + (1 - beta1) g;  v <- beta2 v + (1 - beta2) g^2;  p <- keep p - size * m / (root sqrt(v) + eps)
-__device__ __forceinline__ void adamw_element(float& p, float g, float& m, float& v, const Consts& k, const Factors& f) {
+// The step with 8-bit moments has about as many instructions as it has bytes: EXACT = false takes the quotient from v_sqrt and v_rcp, each
+// good to 2^-24, in place of the exactly rounded sequences (302 M bf16: step and unpacking 985 -> 884 us).  v_sqrt takes a v below 2^-126
+// for 0: beside eps >= 2^-39 / sqrt(1 - beta2), which is 2^-39 root or more, that is below 2^-24 of the denominator.  A smaller eps takes
+// the exact sequences.
+template <bool EXACT> __device__ __forceinline__ void adamw_element(float& p, float g, float& m, float& v, const Consts& k, const Factors& f) {
   m = m * k.beta1 + g * k.one_beta1;
   v = v * k.beta2 + (g * g) * k.one_beta2;
-  p = p * f.keep - (m / (sqrtf(v) * f.root + k.eps)) * f.size;
-}
-__device__ __forceinline__ void adamw8_element(float& p, float g, float& m, float& v, const Consts& k, const Factors& f) {
-  m = m * k.beta1 + g * k.one_beta1;
-  v = v * k.beta2 + (g * g) * k.one_beta2;
-  p = p * f.keep - quotient8(m, v, f.root, k.eps) * f.size;
+  const float q = EXACT ? m / (sqrtf(v) * f.root + k.eps) : m * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v) * f.root + k.eps);
+  p = p * f.keep - q * f.size;
 }
 
 // ------------------------------------------------------------------------------------------------ AdamW, 32-bit moments
@@ -333,7 +323,7 @@ __global__ __launch_bounds__(kThreads) void adamw_step_kernel(StepTable tab, con
   const int block = (int)blockIdx.x - tab.block0[i];
   const auto single = [&](long q) {
     float xp = (float)p[q], xm = m[q], xv = v[q];
-    adamw_element(xp, (float)g[q] * c, xm, xv, k, f);
+    adamw_element<true>(xp, (float)g[q] * c, xm, xv, k, f);
     p[q] = (T)xp; m[q] = xm; v[q] = xv;
   };
   if (block == 0 && (int)threadIdx.x < head) single(threadIdx.x);
@@ -345,7 +335,7 @@ __global__ __launch_bounds__(kThreads) void adamw_step_kernel(StepTable tab, con
     load_f32<float, N>(v + e, xv);
     load_f32<T, N>(p + e, xp);
 #pragma unroll
-    for (int j = 0; j < N; ++j) adamw_element(xp[j], xg[j] * c, xm[j], xv[j], k, f);
+    for (int j = 0; j < N; ++j) adamw_element<true>(xp[j], xg[j] * c, xm[j], xv[j], k, f);
     store_f32<T, N>(p + e, xp);
     store_f32<float, N>(m + e, xm);
     store_f32<float, N>(v + e, xv);
@@ -379,6 +369,23 @@ __device__ __forceinline__ float decode_v(unsigned code, int base) {
   unsigned bits = code ? (code + (unsigned)(base & 0x3FFF)) << 20 : 0u;
   if ((base & kNanFlag) && code == 255u) bits = 0x7FC00000u;
   return __uint_as_float(bits);
+}
+// four codes each; base: the block's two, the same for the whole wave
+__device__ __forceinline__ void decode4(unsigned cm, unsigned cv, int base, float (&m)[4], float (&v)[4]) {
+  const unsigned bm = (unsigned)base & 0x3FFFu, bv = ((unsigned)base >> 16) & 0x3FFFu;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const unsigned a = (cm >> (8 * j)) & 127u, b = (cv >> (8 * j)) & 255u, sign = (cm << (24 - 8 * j)) & 0x80000000u;
+    m[j] = __uint_as_float((a ? (a + bm) << 20 : 0u) | sign);
+    v[j] = __uint_as_float(b ? (b + bv) << 20 : 0u);
+  }
+  if (__builtin_expect(base & (kNanFlag | kNanFlag << 16), 0)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      m[j] = decode_m((cm >> (8 * j)) & 255u, base & 0xFFFF);
+      v[j] = decode_v((cv >> (8 * j)) & 255u, base >> 16);
+    }
+  }
 }
 
 struct Step8Table {
@@ -445,31 +452,22 @@ __device__ __forceinline__ int codes4(const float (&m)[4], const float (&v)[4], 
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int qm = (int)(q[j] & 0xFFFFu), qv = (int)(q[j] >> 16);
-    int lm = max(qm - bm, 0), lv = max(qv - bv, v[j] > 0.f ? 1 : 0);
+    int lm = max(qm - bm, 0), lv = max(qv - bv, (int)min(__float_as_uint(v[j]), 1u));
     if (flag) {
       lm = qm >= kInfLevel ? 127 : lm;
       lv = qv >= kInfLevel ? 255 : lv;
     }
-    cm |= ((unsigned)lm | (m[j] < 0.f ? 128u : 0u)) << (8 * j);
+    cm |= ((unsigned)lm | ((__float_as_uint(m[j]) >> 24) & 128u)) << (8 * j);
     cv |= (unsigned)lv << (8 * j);
   }
   return bm | bv << 16 | flag | flag << 16;
-}
-
-__device__ __forceinline__ void decode4(unsigned cm, unsigned cv, int base, float (&m)[4], float (&v)[4]) {
-  const int bm = base & 0xFFFF, bv = base >> 16;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    m[j] = decode_m((cm >> (8 * j)) & 255u, bm);
-    v[j] = decode_v((cv >> (8 * j)) & 255u, bv);
-  }
 }
 
 typedef unsigned Word __attribute__((aligned(1)));   // four codes, at any address
 
 // A lane has four neighbours of each of the wave's blocks, so that all of the wave's accesses are runs of memory (1 KiB of fp32
 // parameters, 256 bytes of codes), and all loads are on their way before the first is used.
-template <typename T, int WB>
+template <typename T, int WB, bool EXACT>
 __global__ __launch_bounds__(kThreads) void adamw8_step_kernel(Step8Table tab, const Factors* __restrict__ factors,
                                                                const float* __restrict__ clip, int skip_nonfinite, Consts k) {
   const int i = owner(tab.block0, tab.n, blockIdx.x);
@@ -503,7 +501,7 @@ __global__ __launch_bounds__(kThreads) void adamw8_step_kernel(Step8Table tab, c
       float xm[4], xv[4];
       decode4(um[u], uv[u], b[u], xm, xv);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) adamw8_element(xp[u][j], xg[u][j] * c, xm[j], xv[j], k, f);
+      for (int j = 0; j < 4; ++j) adamw_element<EXACT>(xp[u][j], xg[u][j] * c, xm[j], xv[j], k, f);
       store_f32<T, 4>(p + e + u * kBlock, xp[u]);
       const unsigned h = mix32((unsigned)((e + u * kBlock) >> 3) ^ f.key);
       unsigned q[4];
@@ -531,7 +529,7 @@ __global__ __launch_bounds__(kThreads) void adamw8_step_kernel(Step8Table tab, c
         xm[j] = decode_m(cm[e1 + j], b & 0xFFFF);
         xv[j] = decode_v(cv[e1 + j], b >> 16);
         float xp = (float)p[e1 + j];
-        adamw8_element(xp, (float)g[e1 + j] * c, xm[j], xv[j], k, f);
+        adamw_element<EXACT>(xp, (float)g[e1 + j] * c, xm[j], xv[j], k, f);
         p[e1 + j] = (T)xp;
       }
     }
@@ -922,10 +920,11 @@ extern "C" int dtt_adamw8_step(int n, int dtype, void* const* params, const void
   dtt_prof_begin("adamw8", stream);
   if (!prepare(n, dtype, grads, numel, steps, lr, lr_device, weight_decay, ids, seed, beta1, beta2, max_norm, clip, skip_nonfinite, factors,
                stream)) return 0;
+  const bool exact = !(eps >= 0x1p-39 / sqrt(1.0 - beta2));
   Step8Table tab;
   for (int i0 = 0; i0 < n; i0 += tab.n) {
     tab.n = fit(n - i0, kMaxStep8, numel + i0);
-    const bool four = four_blocks(tab.n, numel + i0);
+    const bool four = !exact && four_blocks(tab.n, numel + i0);
     int blocks = 0;
     for (int j = 0; j < tab.n; ++j) {
       const int i = i0 + j;
@@ -937,9 +936,15 @@ extern "C" int dtt_adamw8_step(int n, int dtype, void* const* params, const void
     const auto launch = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kThreads), 0, stream, tab, factors + i0, clip, skip_nonfinite, k);
     };
-    if (dtype == kF32) four ? launch(adamw8_step_kernel<float, 4>) : launch(adamw8_step_kernel<float, 1>);
-    else if (dtype == kBf16) four ? launch(adamw8_step_kernel<__bf16, 4>) : launch(adamw8_step_kernel<__bf16, 1>);
-    else four ? launch(adamw8_step_kernel<_Float16, 4>) : launch(adamw8_step_kernel<_Float16, 1>);
+    const auto shape = [&](auto type) {
+      using T = decltype(type);
+      if (exact) launch(adamw8_step_kernel<T, 1, true>);
+      else if (four) launch(adamw8_step_kernel<T, 4, false>);
+      else launch(adamw8_step_kernel<T, 1, false>);
+    };
+    if (dtype == kF32) shape(float());
+    else if (dtype == kBf16) shape(__bf16());
+    else shape(_Float16());
     DTT_CHECK_LAUNCH("adamw8_step_kernel");
   }
   dtt_prof_end("adamw8", stream);
