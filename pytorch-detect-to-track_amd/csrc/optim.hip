@@ -465,9 +465,14 @@ __device__ __forceinline__ int codes4(const float (&m)[4], const float (&v)[4], 
 
 typedef unsigned Word __attribute__((aligned(1)));   // four codes, at any address
 
+// Codes of up to kKeepCodes bytes in a call are left in the caches for whoever reads them next (KEEP), more of them pass by: as lines that
+// wait to be written back they would only be in the way.  The step itself takes as long either way; unpacking behind it, us, kept /
+// passing by: 110 MB of codes 53 / 62, 604 MB 346 / 295.
+constexpr long kKeepCodes = 256L << 20;
+
 // A lane has four neighbours of each of the wave's blocks, so that all of the wave's accesses are runs of memory (1 KiB of fp32
 // parameters, 256 bytes of codes), and all loads are on their way before the first is used.
-template <typename T, int WB, bool EXACT>
+template <typename T, int WB, bool EXACT, bool KEEP>
 __global__ __launch_bounds__(kThreads) void adamw8_step_kernel(Step8Table tab, const Factors* __restrict__ factors,
                                                                const float* __restrict__ clip, int skip_nonfinite, Consts k) {
   const int i = owner(tab.block0, tab.n, blockIdx.x);
@@ -490,8 +495,10 @@ __global__ __launch_bounds__(kThreads) void adamw8_step_kernel(Step8Table tab, c
     int b[WB];
 #pragma unroll
     for (int u = 0; u < WB; ++u) {
-      um[u] = *reinterpret_cast<const Word*>(cm + e + u * kBlock);
-      uv[u] = *reinterpret_cast<const Word*>(cv + e + u * kBlock);
+      const Word* wm = reinterpret_cast<const Word*>(cm + e + u * kBlock);
+      const Word* wv = reinterpret_cast<const Word*>(cv + e + u * kBlock);
+      um[u] = KEEP ? *wm : __builtin_nontemporal_load(wm);
+      uv[u] = KEEP ? *wv : __builtin_nontemporal_load(wv);
       load_f32<T, 4>(g + e + u * kBlock, xg[u]);
       load_f32<T, 4>(p + e + u * kBlock, xp[u]);
       b[u] = base[u];
@@ -508,8 +515,13 @@ __global__ __launch_bounds__(kThreads) void adamw8_step_kernel(Step8Table tab, c
       levels4(xm, xv, (lane & 1) ? h * 9u : h, 2u * h, q);
       unsigned wm, wv;
       b[u] = codes4(xm, xv, q, wm, wv);
-      *reinterpret_cast<Word*>(cm + e + u * kBlock) = wm;
-      *reinterpret_cast<Word*>(cv + e + u * kBlock) = wv;
+      if (KEEP) {
+        *reinterpret_cast<Word*>(cm + e + u * kBlock) = wm;
+        *reinterpret_cast<Word*>(cv + e + u * kBlock) = wv;
+      } else {
+        __builtin_nontemporal_store(wm, reinterpret_cast<Word*>(cm + e + u * kBlock));
+        __builtin_nontemporal_store(wv, reinterpret_cast<Word*>(cv + e + u * kBlock));
+      }
     }
     if (lane == 0) {
 #pragma unroll
@@ -597,6 +609,10 @@ template <typename T, int WB> __global__ __launch_bounds__(kThreads) void unpack
 }
 
 // ------------------------------------------------------------------------------------------------ host side
+// (kernel arguments are 4 KiB at most; beside a table a launch passes under 100 bytes)
+static_assert(sizeof(NormTable) <= 3968 && sizeof(ScaleTable) <= 3968 && sizeof(PrepareTable) <= 3968 && sizeof(StepTable) <= 3968 &&
+              sizeof(Step8Table) <= 3968 && sizeof(UnpackTable) <= 3968, "tensors per launch");
+
 int type_bytes(int dtype) { return dtype == kF32 ? 4 : 2; }
 
 // Buffers that a call writes must not meet anything else that it reads or writes (the same parameter twice, a moment that is a
@@ -921,6 +937,9 @@ extern "C" int dtt_adamw8_step(int n, int dtype, void* const* params, const void
   if (!prepare(n, dtype, grads, numel, steps, lr, lr_device, weight_decay, ids, seed, beta1, beta2, max_norm, clip, skip_nonfinite, factors,
                stream)) return 0;
   const bool exact = !(eps >= 0x1p-39 / sqrt(1.0 - beta2));
+  long codes = 0;
+  for (int i = 0; i < n; ++i) codes += 2 * numel[i];
+  const bool keep = codes <= kKeepCodes;
   Step8Table tab;
   for (int i0 = 0; i0 < n; i0 += tab.n) {
     tab.n = fit(n - i0, kMaxStep8, numel + i0);
@@ -938,9 +957,10 @@ extern "C" int dtt_adamw8_step(int n, int dtype, void* const* params, const void
     };
     const auto shape = [&](auto type) {
       using T = decltype(type);
-      if (exact) launch(adamw8_step_kernel<T, 1, true>);
-      else if (four) launch(adamw8_step_kernel<T, 4, false>);
-      else launch(adamw8_step_kernel<T, 1, false>);
+      if (exact) launch(adamw8_step_kernel<T, 1, true, true>);
+      else if (!four) launch(adamw8_step_kernel<T, 1, false, true>);
+      else if (keep) launch(adamw8_step_kernel<T, 4, false, true>);
+      else launch(adamw8_step_kernel<T, 4, false, false>);
     };
     if (dtype == kF32) shape(float());
     else if (dtype == kBf16) shape(__bf16());

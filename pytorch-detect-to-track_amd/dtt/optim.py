@@ -488,6 +488,8 @@ class GroupedAdamW(torch.optim.Optimizer):
             if i not in saved:
                 continue
             src = saved[i]
+            if "step" not in src or not ("exp_avg" in src or "exp_avg_code" in src):
+                raise ValueError("GroupedAdamW: not a state of AdamW or Adam (it holds %s)" % sorted(src))
             st = self.state[p]
             t = src["step"]
             st["step"] = torch.as_tensor(t).detach().clone().to(device=p.device, dtype=torch.float32).reshape(())

@@ -136,6 +136,10 @@ def test_refusals_before_any_gpu_work():
     with pytest.raises(ValueError, match="amsgrad"):
         ref = torch.optim.AdamW([w], amsgrad=True)
         opt.load_state_dict(ref.state_dict())
+    sgd = torch.optim.SGD([w], lr=0.1, momentum=0.9)
+    sgd.step()
+    with pytest.raises(ValueError, match="not a state of AdamW"):
+        opt.load_state_dict(sgd.state_dict())
 
 
 def test_library_refuses_bad_arguments_without_a_gpu():
