@@ -98,6 +98,24 @@ def test_norm_of_mixed_types_many_tensors_and_extreme_values():
     assert float(grad_norm([torch.empty(0, device=DEV)])) == 0.0
 
 
+def test_clip_of_many_tensors_of_mixed_types():
+    """More tensors than a launch holds, empty ones among them, one norm over three types; within the limit nothing is written."""
+    from dtt.optim import clip_grads_
+    rs = np.random.RandomState(4)
+    types = list(HALF)
+    grads = [torch.from_numpy(rs.randn(int(rs.randint(0, 2000)) if i % 9 else 0).astype(np.float32)).to(DEV).to(types[i % 3]) for i in range(401)]
+    old = [f64(g) for g in grads]
+    norm, c = oo.norm_and_factor(old, 10.0)
+    assert c < 1
+    first = [g.clone() for g in grads]
+    assert abs(float(clip_grads_(grads, 1e6)) - norm) <= norm * 2.0 ** -23 and all(torch.equal(a, b) for a, b in zip(grads, first))
+    assert abs(float(clip_grads_(grads, 10.0)) - norm) <= norm * 2.0 ** -23
+    for g, o in zip(grads, old):
+        assert (np.abs(f64(g) - o * c) <= np.abs(o * c) * (2 * oo.U + HALF[g.dtype]) + SMALLEST[g.dtype]).all()
+    empty = [torch.empty(0, device=DEV), torch.empty(0, 3, device=DEV, dtype=torch.bfloat16)]
+    assert float(clip_grads_(empty, 1.0)) == 0.0
+
+
 def test_clip_grad_norm_over_parameters():
     from dtt.optim import clip_grad_norm_
     torch.manual_seed(0)
@@ -599,6 +617,42 @@ def test_class_matches_torch_adamw_and_exchanges_checkpoints():
     ob2.load_state_dict(copy.deepcopy(sa))
     both(10, 10, oa2, ob2)
     assert float(ob2.state[next(b.parameters())]["step"]) == 20
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_one_norm_over_groups_of_different_betas_and_types(bits):
+    """Two (betas, eps) and two element types in one optimizer with a limit: one norm over all gradients; the same update as the
+    operators called with that norm."""
+    from dtt.optim import GroupedAdamW, adamw8_, adamw_, blocks_of, grad_norm
+    torch.manual_seed(8)
+    shapes = [((70, 9), torch.float32), ((300,), torch.bfloat16), ((5, 5), torch.float32), ((1000,), torch.bfloat16)]
+    ps = [torch.nn.Parameter(torch.randn(*s, device=DEV).to(t)) for s, t in shapes]
+    for p in ps:
+        p.grad = torch.randn_like(p)
+    ps[0].grad = torch.full((1, 1), 0.25, device=DEV).expand(70, 9)          # a broadcast gradient
+    betas = [(0.9, 0.999), (0.9, 0.999), (0.8, 0.9), (0.8, 0.9)]
+    qs = [p.detach().clone() for p in ps]
+    opt = GroupedAdamW([{"params": [p], "betas": b} for p, b in zip(ps, betas)], lr=1e-2, weight_decay=0.1, state_bits=bits, max_norm=0.5,
+                       skip_nonfinite=True, seed=11)
+    opt.step()
+    gs = [p.grad.contiguous() for p in ps]
+    norm = grad_norm(gs)
+    assert torch.equal(opt.grad_norm, norm) and abs(float(norm) - math.sqrt(sum(float(g.double().square().sum()) for g in gs))) <= float(norm) * 2.0 ** -23
+    clip = torch.stack([norm, (0.5 / (norm.double() + 1e-6)).float()])
+    for first in (0, 2):
+        at = [first, first + 1]
+        s = [torch.zeros((), device=DEV) for _ in at]
+        common = dict(lr=1e-2, betas=betas[first], weight_decay=0.1, clip=clip, skip_nonfinite=True)
+        if bits == 32:
+            out = adamw_([qs[i] for i in at], [gs[i] for i in at], *[[torch.zeros_like(qs[i], dtype=torch.float32) for i in at] for _ in range(2)], s, **common)
+        else:
+            out = adamw8_([qs[i] for i in at], [gs[i] for i in at], *[[torch.zeros_like(qs[i], dtype=torch.uint8) for i in at] for _ in range(2)],
+                          [torch.zeros(blocks_of(qs[i].numel()), 2, dtype=torch.int16, device=DEV) for i in at], s, seed=11, ids=at, **common)
+        assert torch.equal(out, norm)
+    # the factor of the operators' call was rounded from the rounded norm: a last place of the clipped gradient, which the first step of
+    # Adam (g / |g|) does not see beyond 32 U of its size, and half a step of the type
+    for p, q in zip(ps, qs):
+        assert ((p.detach().float() - q.float()).abs() <= 1e-2 * 64 * oo.U + q.float().abs() * (2 * HALF[p.dtype])).all()
 
 
 @pytest.mark.parametrize("bits", [32, 8])
