@@ -1,6 +1,6 @@
 // dtt._tensorlist: what a multi-tensor call has to know of its lists of tensors -- addresses, element counts, types, device,
 // memory order -- read in one pass over each list.  From Python this costs about 4 us per parameter of an AdamW step (five
-// tensors with seven questions each); a step of 300 small tensors takes the GPU 30 us.
+// tensors with seven questions each): 1.1 ms for 301 small tensors, whose kernels take 56 us.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <torch/csrc/autograd/python_variable.h>

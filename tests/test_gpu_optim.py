@@ -619,6 +619,21 @@ def test_class_matches_torch_adamw_and_exchanges_checkpoints():
     assert float(ob2.state[next(b.parameters())]["step"]) == 20
 
 
+def test_a_rate_in_device_memory_survives_a_checkpoint(tmp_path):
+    from dtt.optim import GroupedAdamW
+    w = torch.nn.Parameter(torch.ones(50, device=DEV))
+    opt = GroupedAdamW([w], lr=torch.full((), 0.25, device=DEV), weight_decay=0.0)
+    w.grad = torch.ones_like(w)
+    opt.step()
+    torch.save(opt.state_dict(), tmp_path / "o.pth")
+    v = torch.nn.Parameter(w.detach().clone())
+    again = GroupedAdamW([v], lr=0.5, weight_decay=0.0)
+    again.load_state_dict(torch.load(tmp_path / "o.pth", map_location="cpu"))
+    v.grad = torch.ones_like(v)
+    opt.step(); again.step()
+    assert again.param_groups[0]["lr"].device == v.device and torch.equal(v, w)
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_one_norm_over_groups_of_different_betas_and_types(bits):
     """Two (betas, eps) and two element types in one optimizer with a limit: one norm over all gradients; the same update as the
