@@ -263,19 +263,12 @@ def _plain(st):
 
 
 # ------------------------------------------------------------------------------------------------ the framework's form
-_optim = None
-
-
 def _framework():
-    """dtt.optim, looked up once (a program has imported it before it takes its first step)."""
-    global _optim
-    if _optim is None:
-        root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "pytorch-detect-to-track_amd")
-        if root not in sys.path:
-            sys.path.insert(0, root)
-        from dtt import optim
-        _optim = optim
-    return _optim
+    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "pytorch-detect-to-track_amd")
+    if root not in sys.path:
+        sys.path.insert(0, root)
+    from dtt import optim
+    return optim
 
 
 def _own(st):
