@@ -22,6 +22,40 @@ import torch.distributed as dist
 from torch import nn
 
 
+class _Staged:
+    """The handle of an all-reduce whose tensor went through host memory: wait() brings the sum back."""
+
+    def __init__(self, work, host, tensor):
+        self.work, self.host, self.tensor = work, host, tensor
+
+    def wait(self):
+        self.work.wait()
+        self.tensor.copy_(self.host)
+
+
+def _through_host(t, group):
+    """gloo is given host memory only: its collectives on device tensors hang where several ranks share a GPU."""
+    backend = dist.get_backend(group)
+    return t.device.type != "cpu" and (backend == "gloo" or t.device.type + ":gloo" in backend)
+
+
+def _broadcast(t, src, group):
+    if _through_host(t, group):
+        host = t.cpu()
+        dist.broadcast(host, src=src, group=group)
+        t.copy_(host)
+    else:
+        dist.broadcast(t, src=src, group=group)
+
+
+def _all_reduce_async(t, group):
+    """The sum over ranks in place of t, once the returned handle's wait() is through."""
+    if _through_host(t, group):
+        host = t.cpu()
+        return _Staged(dist.all_reduce(host, op=dist.ReduceOp.SUM, group=group, async_op=True), host, t)
+    return dist.all_reduce(t, op=dist.ReduceOp.SUM, group=group, async_op=True)
+
+
 def _bucket_view(flat, off, p):
     """Slice of a flat bucket shaped and laid out like p (channels-last parameters get a channels-last view, so
     gradient accumulation and the multi-tensor optimizer never mix layouts)."""
@@ -56,7 +90,7 @@ class DataParallelSnippets(nn.Module):
                 if t.data_ptr() in seen or not t.is_floating_point():
                     continue
                 seen.add(t.data_ptr())
-                dist.broadcast(t.data, src=0, group=self.group)
+                _broadcast(t.data, 0, self.group)
 
     def _build_buckets(self, bucket_bytes):
         params, seen = [], set()
@@ -116,7 +150,7 @@ class DataParallelSnippets(nn.Module):
         if dst:
             torch._foreach_copy_(dst, src)
         if dist.is_initialized():   # (force_buckets without a process group: buckets and hooks only)
-            self._handles.append(dist.all_reduce(flat, op=dist.ReduceOp.SUM, group=self.group, async_op=True))
+            self._handles.append(_all_reduce_async(flat, self.group))
 
     def _make_hook(self, bucket_index):
         def hook(param):
@@ -175,7 +209,7 @@ class DataParallelSnippets(nn.Module):
         for _ in range(repeats):
             torch.cuda.synchronize(dev)
             t0 = time.perf_counter()
-            hs = [dist.all_reduce(flat, op=dist.ReduceOp.SUM, group=self.group, async_op=True) for flat, _ in self._buckets]
+            hs = [_all_reduce_async(flat, self.group) for flat, _ in self._buckets]
             for h in hs:
                 h.wait()
             torch.cuda.synchronize(dev)
@@ -240,7 +274,7 @@ def broadcast_module_state(module, process_group=None, src=0):
             if t.data_ptr() in seen or not t.is_floating_point():
                 continue
             seen.add(t.data_ptr())
-            dist.broadcast(t.data, src=src, group=process_group)
+            _broadcast(t.data, src, process_group)
     return module
 
 
