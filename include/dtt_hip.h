@@ -595,7 +595,8 @@ int dtt_tube_link(const float* dets, int det_stride, const int* n, const float* 
  * array is a HOST array of n entries holding device pointers / counts / rates; a tensor is a dense run of numel elements in
  * memory order (the buffers of one tensor in the same order), at any element-aligned address.  dtype: 0 = fp32, 1 = bf16, 2 = fp16.
  * n = 0 and empty tensors are allowed.  All state, the step counters among it, is in device memory: a captured call counts on with
- * every replay.  Buffers that a call writes must not overlap anything else it is given (refused: status 0).
+ * every replay.  Buffers that a call writes (norm and factor, workspace among them) must not overlap anything else it is given
+ * (learning rates in device memory among it; refused: status 0).
  *
  * dtt_grad_norm: out[0] = sqrt(sum of all squares), out[1] = min(1, max_norm / (out[0] + 1e-6)) -- the factor that brings the
  * gradients to the limit; max_norm = infinity asks for the norm alone (factor 1).  Squares and sums in 64 bits, in a fixed order.

@@ -616,7 +616,7 @@ static_assert(sizeof(NormTable) <= 3968 && sizeof(ScaleTable) <= 3968 && sizeof(
 int type_bytes(int dtype) { return dtype == kF32 ? 4 : 2; }
 
 // Buffers that a call writes must not meet anything else that it reads or writes (the same parameter twice, a moment that is a
-// view of another, a shared step counter): the workgroups run in no order.
+// view of another, a shared step counter, a learning rate inside a parameter): the workgroups run in no order.
 struct Spans {
   struct Span {
     uintptr_t lo, hi;   // twice the addresses; hi's lowest bit says "written"
@@ -725,9 +725,16 @@ extern "C" int dtt_grad_norm(int n, const void* const* grads, const long* numel,
                              void* workspace, size_t workspace_bytes, void* stream_) {
   hipStream_t stream = static_cast<hipStream_t>(stream_);
   if (!check_grads("grad_norm", n, grads, numel, dtypes)) return 0;
-  DTT_REQUIRE(out && workspace && aligned_to(workspace, 8), "grad_norm: null or unaligned pointer");
+  DTT_REQUIRE(out && aligned_to(out, 4) && workspace && aligned_to(workspace, 8), "grad_norm: null or unaligned pointer");
   DTT_REQUIRE(max_norm >= 0.0, "grad_norm: max_norm must not be negative");
-  DTT_REQUIRE(workspace_bytes >= dtt_grad_norm_workspace_bytes(n, numel), "grad_norm: workspace too small");
+  const size_t need = dtt_grad_norm_workspace_bytes(n, numel);
+  DTT_REQUIRE(workspace_bytes >= need, "grad_norm: workspace too small");
+  Spans spans(n + 2L);
+  DTT_REQUIRE(spans.s, "grad_norm: out of host memory");
+  for (int i = 0; i < n; ++i) spans.add(grads[i], numel[i] * type_bytes(dtypes[i]), false);
+  spans.add(out, 8, true);
+  spans.add(workspace, (long)need, true);
+  DTT_REQUIRE(!spans.clash(), "grad_norm: the result, the workspace or a gradient share memory");
   double* partial = static_cast<double*>(workspace);
   dtt_prof_begin("grad_norm", stream);
   const int blocks = norm_partials(n, grads, numel, dtypes, 0, partial, stream);
@@ -742,13 +749,16 @@ extern "C" int dtt_grad_clip(int n, void* const* grads, const long* numel, const
                              size_t workspace_bytes, void* stream_) {
   hipStream_t stream = static_cast<hipStream_t>(stream_);
   if (!check_grads("grad_clip", n, grads, numel, dtypes)) return 0;
-  DTT_REQUIRE(out && workspace && aligned_to(workspace, 8), "grad_clip: null or unaligned pointer");
+  DTT_REQUIRE(out && aligned_to(out, 4) && workspace && aligned_to(workspace, 8), "grad_clip: null or unaligned pointer");
   DTT_REQUIRE(max_norm >= 0.0, "grad_clip: max_norm must not be negative");
-  DTT_REQUIRE(workspace_bytes >= dtt_grad_norm_workspace_bytes(n, numel), "grad_clip: workspace too small");
-  Spans spans(n);
+  const size_t need = dtt_grad_norm_workspace_bytes(n, numel);
+  DTT_REQUIRE(workspace_bytes >= need, "grad_clip: workspace too small");
+  Spans spans(n + 2L);
   DTT_REQUIRE(spans.s, "grad_clip: out of host memory");
   for (int i = 0; i < n; ++i) spans.add(grads[i], numel[i] * type_bytes(dtypes[i]), true);
-  DTT_REQUIRE(!spans.clash(), "grad_clip: two gradients share memory");
+  spans.add(out, 8, true);
+  spans.add(workspace, (long)need, true);
+  DTT_REQUIRE(!spans.clash(), "grad_clip: two of the gradients, the result or the workspace share memory");
   double* partial = static_cast<double*>(workspace);
   dtt_prof_begin("grad_clip", stream);
   NormPart part;
@@ -789,27 +799,33 @@ namespace {
 
 // what both steps check of their arguments; the buffers' spans are collected for the overlap check
 int check_step(const char* what, int n, int dtype, void* const* params, const void* const* grads, const long* numel, float* const* steps,
-               const double* lr, const double* decay, double beta1, double beta2, double eps, double max_norm, const float* clip,
+               const double* lr, const float* const* lr_device, const double* decay, double beta1, double beta2, double eps, double max_norm, const float* clip,
                int skip_nonfinite, const void* workspace, size_t workspace_bytes, Spans& spans) {
   DTT_REQUIRE(n >= 0 && (n == 0 || (params && grads && numel && steps && lr && decay)), "%s: null pointer", what);
   DTT_REQUIRE(dtype >= kF32 && dtype <= kF16, "%s: unknown element type %d", what, dtype);
   DTT_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "%s: betas must lie in [0, 1)", what);
   DTT_REQUIRE(eps >= 0.0, "%s: eps must not be negative", what);
   DTT_REQUIRE(max_norm == max_norm, "%s: max_norm is not a number", what);
+  DTT_REQUIRE(aligned_to(clip, 4), "%s: unaligned norm and factor", what);
   DTT_REQUIRE(clip || (!skip_nonfinite && max_norm < 0.0), "%s: clipping and skip_nonfinite need a place for norm and factor", what);
   DTT_REQUIRE(spans.s, "%s: out of host memory", what);
   const int es = type_bytes(dtype);
   for (int i = 0; i < n; ++i) {
     DTT_REQUIRE(numel[i] >= 0 && numel[i] <= kMaxNumel, "%s: tensor %d: bad element count", what, i);
     DTT_REQUIRE(steps[i] && aligned_to(steps[i], 4), "%s: tensor %d: null or unaligned step counter", what, i);
+    DTT_REQUIRE(!lr_device || aligned_to(lr_device[i], 4), "%s: tensor %d: unaligned learning rate", what, i);
     DTT_REQUIRE(lr[i] >= 0.0 && decay[i] >= 0.0, "%s: tensor %d: learning rate and weight decay must not be negative", what, i);
     DTT_REQUIRE(numel[i] == 0 || (params[i] && grads[i] && aligned_to(params[i], es) && aligned_to(grads[i], es)),
                 "%s: tensor %d: null or unaligned pointer", what, i);
   }
-  DTT_REQUIRE(workspace && aligned_to(workspace, 16) && workspace_bytes >= dtt_adamw_workspace_bytes(n, numel), "%s: workspace too small or unaligned", what);
+  const size_t need = dtt_adamw_workspace_bytes(n, numel);
+  DTT_REQUIRE(workspace && aligned_to(workspace, 16) && workspace_bytes >= need, "%s: workspace too small or unaligned", what);
   for (int i = 0; i < n; ++i) spans.add(params[i], numel[i] * es, true);
   for (int i = 0; i < n; ++i) spans.add(grads[i], numel[i] * es, false);
   for (int i = 0; i < n; ++i) spans.add(steps[i], 4, true);
+  for (int i = 0; lr_device && i < n; ++i) spans.add(lr_device[i], lr_device[i] ? 4 : 0, false);
+  spans.add(clip, clip ? 8 : 0, max_norm >= 0.0);
+  spans.add(workspace, (long)need, true);
   return 1;
 }
 
@@ -874,8 +890,8 @@ extern "C" int dtt_adamw_step(int n, int dtype, void* const* params, const void*
                               const float* const* lr_device, const double* weight_decay, double beta1, double beta2, double eps,
                               double max_norm, float* clip, int skip_nonfinite, void* workspace, size_t workspace_bytes, void* stream_) {
   hipStream_t stream = static_cast<hipStream_t>(stream_);
-  Spans spans(5L * (n > 0 ? n : 0));
-  if (!check_step("adamw", n, dtype, params, grads, numel, steps, lr, weight_decay, beta1, beta2, eps, max_norm, clip, skip_nonfinite, workspace,
+  Spans spans(6L * (n > 0 ? n : 0) + 2);
+  if (!check_step("adamw", n, dtype, params, grads, numel, steps, lr, lr_device, weight_decay, beta1, beta2, eps, max_norm, clip, skip_nonfinite, workspace,
                   workspace_bytes, spans)) return 0;
   DTT_REQUIRE(n == 0 || (exp_avgs && exp_avg_sqs), "adamw: null pointer");
   for (int i = 0; i < n; ++i) {
@@ -884,7 +900,7 @@ extern "C" int dtt_adamw_step(int n, int dtype, void* const* params, const void*
   }
   for (int i = 0; i < n; ++i) spans.add(exp_avgs[i], numel[i] * 4, true);
   for (int i = 0; i < n; ++i) spans.add(exp_avg_sqs[i], numel[i] * 4, true);
-  DTT_REQUIRE(!spans.clash(), "adamw: two of the tensors share memory");
+  DTT_REQUIRE(!spans.clash(), "adamw: two of the buffers share memory");
   Factors* factors = static_cast<Factors*>(workspace);
   const Consts k = consts(beta1, beta2, eps);
   dtt_prof_begin("adamw", stream);
@@ -919,8 +935,8 @@ extern "C" int dtt_adamw8_step(int n, int dtype, void* const* params, const void
                                unsigned seed, double beta1, double beta2, double eps, double max_norm, float* clip, int skip_nonfinite,
                                void* workspace, size_t workspace_bytes, void* stream_) {
   hipStream_t stream = static_cast<hipStream_t>(stream_);
-  Spans spans(6L * (n > 0 ? n : 0));
-  if (!check_step("adamw8", n, dtype, params, grads, numel, steps, lr, weight_decay, beta1, beta2, eps, max_norm, clip, skip_nonfinite, workspace,
+  Spans spans(7L * (n > 0 ? n : 0) + 2);
+  if (!check_step("adamw8", n, dtype, params, grads, numel, steps, lr, lr_device, weight_decay, beta1, beta2, eps, max_norm, clip, skip_nonfinite, workspace,
                   workspace_bytes, spans)) return 0;
   DTT_REQUIRE(n == 0 || (exp_avgs && exp_avg_sqs && bases), "adamw8: null pointer");
   for (int i = 0; i < n; ++i) {
@@ -930,7 +946,7 @@ extern "C" int dtt_adamw8_step(int n, int dtype, void* const* params, const void
   for (int i = 0; i < n; ++i) spans.add(exp_avgs[i], numel[i], true);
   for (int i = 0; i < n; ++i) spans.add(exp_avg_sqs[i], numel[i], true);
   for (int i = 0; i < n; ++i) spans.add(bases[i], (numel[i] + kBlock - 1) / kBlock * 4, true);
-  DTT_REQUIRE(!spans.clash(), "adamw8: two of the tensors share memory");
+  DTT_REQUIRE(!spans.clash(), "adamw8: two of the buffers share memory");
   Factors* factors = static_cast<Factors*>(workspace);
   const Consts k = consts(beta1, beta2, eps);
   dtt_prof_begin("adamw8", stream);

@@ -1,0 +1,36 @@
+"""The optimizer operators where calls meet, without a GPU: what the library refuses about buffers that meet, checkpoints that are refused,
+learning rates that groups share."""
+import ctypes
+
+import pytest
+
+
+def test_library_refuses_results_rates_and_workspaces_that_meet_a_tensor():
+    """Norm and factor, the workspace and learning rates in device memory are buffers of the call like any other (status 0, nothing launched)."""
+    from dtt import _lib
+    L = _lib.lib()
+    buf = (ctypes.c_double * 4096)()
+    base = ctypes.addressof(buf)
+    P = lambda *a: (ctypes.c_void_p * len(a))(*a)
+    N = lambda *a: (ctypes.c_long * len(a))(*a)
+    D = lambda *a: (ctypes.c_double * len(a))(*a)
+    I = lambda *a: (ctypes.c_int * len(a))(*a)
+    ws = base + 16384
+    for call in (L.dtt_grad_norm, L.dtt_grad_clip):
+        norm = lambda g=base, out=base + 1024, w=ws: call(1, P(g), N(8), I(0), 1.0, out, w, 4096, None)
+        for kw, why in ((dict(out=base), "share memory"), (dict(out=base + 28), "share memory"), (dict(w=base + 24), "share memory"),
+                        (dict(out=ws), "share memory"), (dict(out=base + 1026), "unaligned")):
+            assert norm(**kw) == 0 and why in _lib.last_error(), (kw, _lib.last_error())
+    p, g, m, v, b, s = (base + k for k in (0, 128, 256, 384, 512, 600))
+
+    def step(bits, rate=None, clip=None, w=ws, limit=-1.0):
+        args = [1, 0, P(p), P(g), P(m), P(v)] + ([P(b)] if bits == 8 else []) + [N(16), P(s), D(1e-3), None if rate is None else P(rate), D(0.0)]
+        tail = [0.9, 0.999, 1e-8, limit, clip, 0, w, 4096, None]
+        return L.dtt_adamw8_step(*args, None, 0, *tail) if bits == 8 else L.dtt_adamw_step(*args, *tail)
+    for bits in (32, 8):
+        for kw, why in ((dict(rate=p), "share memory"), (dict(rate=m), "share memory"), (dict(rate=s), "share memory"), (dict(rate=s + 1), "unaligned"),
+                        (dict(clip=p + 4), "share memory"), (dict(clip=s), "share memory"), (dict(clip=g, limit=1.0), "share memory"),
+                        (dict(clip=base + 1024, rate=base + 1028, limit=1.0), "share memory"), (dict(clip=ws + 8, limit=1.0), "share memory"),
+                        (dict(clip=base + 1026, limit=1.0), "unaligned"), (dict(w=m), "share memory"), (dict(w=base - 16), "share memory"),
+                        (dict(rate=ws), "share memory")):
+            assert step(bits, **kw) == 0 and why in _lib.last_error(), (bits, kw, _lib.last_error())
