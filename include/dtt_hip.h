@@ -618,6 +618,12 @@ int dtt_adamw_step(int n, int dtype, void* const* params, const void* const* gra
                    const long* numel, float* const* steps, const double* lr, const float* const* lr_device,
                    const double* weight_decay, double beta1, double beta2, double eps, double max_norm, float* clip,
                    int skip_nonfinite, void* workspace, size_t workspace_bytes, void* stream);
+/* Several calls as one step (tensors of several dtypes, groups of several betas): what the calls would refuse about their tensors, rates and
+ * norm, and buffers that one call writes and another one is given.  Arrays over the tensors of all calls; bases NULL = fp32 moments.
+ * Status 0 = refused; nothing is launched, and nothing has to be undone. */
+int dtt_adamw_check(int n, const int* dtypes, void* const* params, const void* const* grads, const void* const* exp_avgs,
+                    const void* const* exp_avg_sqs, const short* const* bases, const long* numel, float* const* steps,
+                    const double* lr, const float* const* lr_device, const double* weight_decay, const float* clip);
 /* The same step with the moments in 8 bits: codes of numel bytes each, and bases, two int16 (m, v; 4-byte aligned) per 256 elements in memory
  * order (all zero = moments of zero).  A code counts levels of a fixed grid -- eight per power of two, the upper 12 bits of the fp32 --
  * from its block's base: m sign + 7 bits, v 8 bits; bit 14 of a base: the block holds infinities / NaN, whose code is 127 / 255.

@@ -797,35 +797,70 @@ extern "C" size_t dtt_adamw_workspace_bytes(int n, const long* numel) {
 
 namespace {
 
-// what both steps check of their arguments; the buffers' spans are collected for the overlap check
-int check_step(const char* what, int n, int dtype, void* const* params, const void* const* grads, const long* numel, float* const* steps,
-               const double* lr, const float* const* lr_device, const double* decay, double beta1, double beta2, double eps, double max_norm, const float* clip,
-               int skip_nonfinite, const void* workspace, size_t workspace_bytes, Spans& spans) {
-  DTT_REQUIRE(n >= 0 && (n == 0 || (params && grads && numel && steps && lr && decay)), "%s: null pointer", what);
-  DTT_REQUIRE(dtype >= kF32 && dtype <= kF16, "%s: unknown element type %d", what, dtype);
+// The tensors of a step, of one element type (dtypes NULL) or of several; bases NULL: moments in fp32.
+struct StepLists {
+  int n;
+  const int* dtypes;
+  int dtype;
+  void* const* params;
+  const void* const* grads;
+  const void* const* exp_avgs;
+  const void* const* exp_avg_sqs;
+  const short* const* bases;
+  const long* numel;
+  float* const* steps;
+  const double* lr;
+  const float* const* lr_device;
+  const double* decay;
+};
+
+// what a step checks of its tensors, rates and norm; the buffers' spans are collected for the overlap check (spans_of(n) of them at most)
+long spans_of(int n) { return 7L * (n > 0 ? n : 0) + 2; }
+int check_lists(const char* what, const StepLists& l, bool in8bits, const float* clip, bool clip_written, Spans& spans) {
+  DTT_REQUIRE(l.n >= 0 && (l.n == 0 || (l.params && l.grads && l.exp_avgs && l.exp_avg_sqs && l.numel && l.steps && l.lr && l.decay && (l.bases || !in8bits))),
+              "%s: null pointer", what);
+  DTT_REQUIRE(aligned_to(clip, 4), "%s: unaligned norm and factor", what);
+  DTT_REQUIRE(spans.s, "%s: out of host memory", what);
+  const int ms = in8bits ? 1 : 4;
+  for (int i = 0; i < l.n; ++i) {
+    const int dtype = l.dtypes ? l.dtypes[i] : l.dtype;
+    DTT_REQUIRE(dtype >= kF32 && dtype <= kF16, "%s: unknown element type %d", what, dtype);
+    const int es = type_bytes(dtype);
+    DTT_REQUIRE(l.numel[i] >= 0 && l.numel[i] <= kMaxNumel, "%s: tensor %d: bad element count", what, i);
+    DTT_REQUIRE(l.steps[i] && aligned_to(l.steps[i], 4), "%s: tensor %d: null or unaligned step counter", what, i);
+    DTT_REQUIRE(!l.lr_device || aligned_to(l.lr_device[i], 4), "%s: tensor %d: unaligned learning rate", what, i);
+    DTT_REQUIRE(l.lr[i] >= 0.0 && l.decay[i] >= 0.0, "%s: tensor %d: learning rate and weight decay must not be negative", what, i);
+    DTT_REQUIRE(l.numel[i] == 0 || (l.params[i] && l.grads[i] && aligned_to(l.params[i], es) && aligned_to(l.grads[i], es)),
+                "%s: tensor %d: null or unaligned pointer", what, i);
+    DTT_REQUIRE(l.numel[i] == 0 || (l.exp_avgs[i] && l.exp_avg_sqs[i] && aligned_to(l.exp_avgs[i], ms) && aligned_to(l.exp_avg_sqs[i], ms) &&
+                                    (!in8bits || (l.bases[i] && aligned_to(l.bases[i], 4)))),
+                "%s: tensor %d: null or unaligned moment", what, i);
+  }
+  for (int i = 0; i < l.n; ++i) spans.add(l.params[i], l.numel[i] * type_bytes(l.dtypes ? l.dtypes[i] : l.dtype), true);
+  for (int i = 0; i < l.n; ++i) spans.add(l.grads[i], l.numel[i] * type_bytes(l.dtypes ? l.dtypes[i] : l.dtype), false);
+  for (int i = 0; i < l.n; ++i) spans.add(l.steps[i], 4, true);
+  for (int i = 0; i < l.n; ++i) spans.add(l.exp_avgs[i], l.numel[i] * ms, true);
+  for (int i = 0; i < l.n; ++i) spans.add(l.exp_avg_sqs[i], l.numel[i] * ms, true);
+  for (int i = 0; in8bits && i < l.n; ++i) spans.add(l.bases[i], (l.numel[i] + kBlock - 1) / kBlock * 4, true);
+  for (int i = 0; l.lr_device && i < l.n; ++i) spans.add(l.lr_device[i], l.lr_device[i] ? 4 : 0, false);
+  spans.add(clip, clip ? 8 : 0, clip_written);
+  return 1;
+}
+
+// what both steps check
+int check_step(const char* what, const StepLists& l, bool in8bits, double beta1, double beta2, double eps, double max_norm, const float* clip,
+               int skip_nonfinite, const void* workspace, size_t workspace_bytes) {
+  DTT_REQUIRE(l.dtype >= kF32 && l.dtype <= kF16, "%s: unknown element type %d", what, l.dtype);
   DTT_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "%s: betas must lie in [0, 1)", what);
   DTT_REQUIRE(eps >= 0.0, "%s: eps must not be negative", what);
   DTT_REQUIRE(max_norm == max_norm, "%s: max_norm is not a number", what);
-  DTT_REQUIRE(aligned_to(clip, 4), "%s: unaligned norm and factor", what);
   DTT_REQUIRE(clip || (!skip_nonfinite && max_norm < 0.0), "%s: clipping and skip_nonfinite need a place for norm and factor", what);
-  DTT_REQUIRE(spans.s, "%s: out of host memory", what);
-  const int es = type_bytes(dtype);
-  for (int i = 0; i < n; ++i) {
-    DTT_REQUIRE(numel[i] >= 0 && numel[i] <= kMaxNumel, "%s: tensor %d: bad element count", what, i);
-    DTT_REQUIRE(steps[i] && aligned_to(steps[i], 4), "%s: tensor %d: null or unaligned step counter", what, i);
-    DTT_REQUIRE(!lr_device || aligned_to(lr_device[i], 4), "%s: tensor %d: unaligned learning rate", what, i);
-    DTT_REQUIRE(lr[i] >= 0.0 && decay[i] >= 0.0, "%s: tensor %d: learning rate and weight decay must not be negative", what, i);
-    DTT_REQUIRE(numel[i] == 0 || (params[i] && grads[i] && aligned_to(params[i], es) && aligned_to(grads[i], es)),
-                "%s: tensor %d: null or unaligned pointer", what, i);
-  }
-  const size_t need = dtt_adamw_workspace_bytes(n, numel);
+  Spans spans(spans_of(l.n));
+  if (!check_lists(what, l, in8bits, clip, max_norm >= 0.0, spans)) return 0;
+  const size_t need = dtt_adamw_workspace_bytes(l.n, l.numel);
   DTT_REQUIRE(workspace && aligned_to(workspace, 16) && workspace_bytes >= need, "%s: workspace too small or unaligned", what);
-  for (int i = 0; i < n; ++i) spans.add(params[i], numel[i] * es, true);
-  for (int i = 0; i < n; ++i) spans.add(grads[i], numel[i] * es, false);
-  for (int i = 0; i < n; ++i) spans.add(steps[i], 4, true);
-  for (int i = 0; lr_device && i < n; ++i) spans.add(lr_device[i], lr_device[i] ? 4 : 0, false);
-  spans.add(clip, clip ? 8 : 0, max_norm >= 0.0);
   spans.add(workspace, (long)need, true);
+  DTT_REQUIRE(!spans.clash(), "%s: two of the buffers share memory", what);
   return 1;
 }
 
@@ -885,22 +920,25 @@ Consts consts(double beta1, double beta2, double eps) {
 
 }  // namespace
 
+extern "C" int dtt_adamw_check(int n, const int* dtypes, void* const* params, const void* const* grads, const void* const* exp_avgs,
+                               const void* const* exp_avg_sqs, const short* const* bases, const long* numel, float* const* steps,
+                               const double* lr, const float* const* lr_device, const double* weight_decay, const float* clip) {
+  DTT_REQUIRE(n == 0 || dtypes, "adamw_check: null pointer");
+  const StepLists lists = {n, dtypes, 0, params, grads, exp_avgs, exp_avg_sqs, bases, numel, steps, lr, lr_device, weight_decay};
+  Spans spans(spans_of(n));
+  if (!check_lists("adamw_check", lists, bases != nullptr, clip, false, spans)) return 0;
+  DTT_REQUIRE(!spans.clash(), "adamw_check: two of the buffers share memory");
+  return 1;
+}
+
 extern "C" int dtt_adamw_step(int n, int dtype, void* const* params, const void* const* grads, float* const* exp_avgs,
                               float* const* exp_avg_sqs, const long* numel, float* const* steps, const double* lr,
                               const float* const* lr_device, const double* weight_decay, double beta1, double beta2, double eps,
                               double max_norm, float* clip, int skip_nonfinite, void* workspace, size_t workspace_bytes, void* stream_) {
   hipStream_t stream = static_cast<hipStream_t>(stream_);
-  Spans spans(6L * (n > 0 ? n : 0) + 2);
-  if (!check_step("adamw", n, dtype, params, grads, numel, steps, lr, lr_device, weight_decay, beta1, beta2, eps, max_norm, clip, skip_nonfinite, workspace,
-                  workspace_bytes, spans)) return 0;
-  DTT_REQUIRE(n == 0 || (exp_avgs && exp_avg_sqs), "adamw: null pointer");
-  for (int i = 0; i < n; ++i) {
-    DTT_REQUIRE(numel[i] == 0 || (exp_avgs[i] && exp_avg_sqs[i] && aligned_to(exp_avgs[i], 4) && aligned_to(exp_avg_sqs[i], 4)),
-                "adamw: tensor %d: null or unaligned moment", i);
-  }
-  for (int i = 0; i < n; ++i) spans.add(exp_avgs[i], numel[i] * 4, true);
-  for (int i = 0; i < n; ++i) spans.add(exp_avg_sqs[i], numel[i] * 4, true);
-  DTT_REQUIRE(!spans.clash(), "adamw: two of the buffers share memory");
+  const StepLists lists = {n, nullptr, dtype, params, grads, reinterpret_cast<const void* const*>(exp_avgs),
+                           reinterpret_cast<const void* const*>(exp_avg_sqs), nullptr, numel, steps, lr, lr_device, weight_decay};
+  if (!check_step("adamw", lists, false, beta1, beta2, eps, max_norm, clip, skip_nonfinite, workspace, workspace_bytes)) return 0;
   Factors* factors = static_cast<Factors*>(workspace);
   const Consts k = consts(beta1, beta2, eps);
   dtt_prof_begin("adamw", stream);
@@ -935,18 +973,9 @@ extern "C" int dtt_adamw8_step(int n, int dtype, void* const* params, const void
                                unsigned seed, double beta1, double beta2, double eps, double max_norm, float* clip, int skip_nonfinite,
                                void* workspace, size_t workspace_bytes, void* stream_) {
   hipStream_t stream = static_cast<hipStream_t>(stream_);
-  Spans spans(7L * (n > 0 ? n : 0) + 2);
-  if (!check_step("adamw8", n, dtype, params, grads, numel, steps, lr, lr_device, weight_decay, beta1, beta2, eps, max_norm, clip, skip_nonfinite, workspace,
-                  workspace_bytes, spans)) return 0;
-  DTT_REQUIRE(n == 0 || (exp_avgs && exp_avg_sqs && bases), "adamw8: null pointer");
-  for (int i = 0; i < n; ++i) {
-    DTT_REQUIRE(numel[i] == 0 || (exp_avgs[i] && exp_avg_sqs[i] && bases[i] && aligned_to(bases[i], 4)),
-                "adamw8: tensor %d: null or unaligned moment", i);
-  }
-  for (int i = 0; i < n; ++i) spans.add(exp_avgs[i], numel[i], true);
-  for (int i = 0; i < n; ++i) spans.add(exp_avg_sqs[i], numel[i], true);
-  for (int i = 0; i < n; ++i) spans.add(bases[i], (numel[i] + kBlock - 1) / kBlock * 4, true);
-  DTT_REQUIRE(!spans.clash(), "adamw8: two of the buffers share memory");
+  const StepLists lists = {n, nullptr, dtype, params, grads, reinterpret_cast<const void* const*>(exp_avgs),
+                           reinterpret_cast<const void* const*>(exp_avg_sqs), bases, numel, steps, lr, lr_device, weight_decay};
+  if (!check_step("adamw8", lists, true, beta1, beta2, eps, max_norm, clip, skip_nonfinite, workspace, workspace_bytes)) return 0;
   Factors* factors = static_cast<Factors*>(workspace);
   const Consts k = consts(beta1, beta2, eps);
   dtt_prof_begin("adamw8", stream);

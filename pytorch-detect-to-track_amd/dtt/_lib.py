@@ -100,6 +100,7 @@ SIGNATURES = {
     "dtt_grad_norm": (_I, [_I, _P, _P, _P, _D, _P, _P, _Z, _P]),
     "dtt_grad_clip": (_I, [_I, _P, _P, _P, _D, _P, _P, _Z, _P]),
     "dtt_adamw_workspace_bytes": (_Z, [_I, _P]),
+    "dtt_adamw_check": (_I, [_I] + [_P] * 12),
     "dtt_adamw_step": (_I, [_I, _I] + [_P] * 9 + [_D] * 4 + [_P, _I, _P, _Z, _P]),
     "dtt_adamw8_step": (_I, [_I, _I] + [_P] * 11 + [_U] + [_D] * 4 + [_P, _I, _P, _Z, _P]),
     "dtt_adamw8_unpack": (_I, [_I] + [_P] * 4 + [_I, _P, _P, _P]),

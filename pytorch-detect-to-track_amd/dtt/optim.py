@@ -237,8 +237,10 @@ def _mend(what, lists, moment_type):
     return [params, grads] + lists[2:]
 
 
-def _step(what, lists, moment_type, lr, betas, eps, weight_decay, max_norm, skip_nonfinite, clip, seed=0, ids=None):
-    """One step of the lists [params, grads, steps, m, v] (32-bit moments) or [..., bases] (8-bit); returns the norm or None."""
+def _calls(what, lists, moment_type, lr, betas, eps, weight_decay, ids):
+    """(calls, gradients in the parameters' order) of the lists [params, grads, steps, m, v] (32-bit moments) or [..., bases] (8-bit).  A
+    call of the library takes tensors of one element type: (lists, (type, device, addresses of each list, counts), rates, addresses of those
+    in device memory, the tensors among them, decay, (beta1, beta2, eps), ids)."""
     lists = [x if type(x) is list else list(x) for x in lists]
     n = len(lists[0])
     if any(len(x) != n for x in lists) or (ids is not None and len(ids) != n):
@@ -248,57 +250,93 @@ def _step(what, lists, moment_type, lr, betas, eps, weight_decay, max_norm, skip
         raise ValueError("%s: betas must lie in [0, 1) (got %r)" % (what, betas))
     if not eps >= 0.0:
         raise ValueError("%s: eps must not be negative (got %r)" % (what, eps))
+    rates, device_rates, tensors = _rates(what, lr, n)
+    decay = _numbers(what, "weight_decay", weight_decay, n)
+    if n == 0:
+        return [], []
+    coefficients = (beta1, beta2, eps)
+    T = _tensorlist()
+    plain = T.step_lists(lists, moment_type, BLOCK)
+    if plain is not None:
+        return [(lists, plain, rates, device_rates, tensors, decay, coefficients, ids)], lists[1]
+    lists = _mend(what, lists, moment_type)
+    by_type = {}
+    for i, p in enumerate(lists[0]):
+        by_type.setdefault(p.dtype, []).append(i)
+    calls = []
+    for at in by_type.values():
+        part = [[x[i] for i in at] for x in lists]
+        plain = T.step_lists(part, moment_type, BLOCK)
+        if plain is None:
+            raise RuntimeError("%s: the lists changed while they were read" % what)
+        some = None if device_rates is None else array("Q", [device_rates[i] for i in at])
+        calls.append((part, plain, array("d", [rates[i] for i in at]), some, tensors, array("d", [decay[i] for i in at]), coefficients,
+                      at if ids is None else [ids[i] for i in at]))
+    return calls, lists[1]
+
+
+def _check_together(what, calls, moment_type, clip):
+    """Several calls are one step: all that one of them would refuse is refused before the first."""
+    join = lambda parts: b"".join(parts)
+    lists, plain, rates, device_rates, _, decay, _, _ = zip(*calls)
+    sizes = [len(x[0]) for x in lists]
+    types, _, ptrs, counts = zip(*plain)
+    p, g, s, m, v = (join(x[k] for x in ptrs) for k in range(5))
+    on_device = None
+    if any(x is not None for x in device_rates):
+        on_device = join(bytes(8 * n) if x is None else x.tobytes() for n, x in zip(sizes, device_rates))
+    check(_lib.lib().dtt_adamw_check(sum(sizes), join(array("i", [t]).tobytes() * n for n, t in zip(sizes, types)), p, g, m, v,
+                                     None if moment_type == 0 else join(x[5] for x in ptrs), join(counts), s, join(x.tobytes() for x in rates),
+                                     on_device, join(x.tobytes() for x in decay), None if clip is None else clip.data_ptr()), what)
+
+
+def _step(what, jobs, moment_type, max_norm, skip_nonfinite, clip, seed=0):
+    """One step of all jobs, each (lists, lr, betas, eps, weight_decay, ids) as _calls takes them, under one norm: done or refused as a
+    whole.  Returns the norm or None."""
     if max_norm is not None:
         max_norm = _limit(what, max_norm)
     if clip is not None and (max_norm is not None or clip.dtype != torch.float32 or tuple(clip.shape) != (2,) or not clip.is_contiguous()):
         raise ValueError("%s: clip is norm and factor, two float32, and stands in place of max_norm" % what)
-    rates, device_rates, extra = _rates(what, lr, n)
-    decay = _numbers(what, "weight_decay", weight_decay, n)
-    if n == 0:
+    calls, grads = [], []
+    for job in jobs:
+        more, own = _calls(what, job[0], moment_type, *job[1:])
+        calls = calls + more if calls else more
+        grads = grads + own if grads else own
+    if not calls:
         return None
-    T = _tensorlist()
-    plain = T.step_lists(lists, moment_type, BLOCK)
-    if plain is None:
-        lists = _mend(what, lists, moment_type)
-        by_type = {}
-        for i, p in enumerate(lists[0]):
-            by_type.setdefault(p.dtype, []).append(i)
-        if len(by_type) > 1:     # one norm over all of them, one call for each type
-            if clip is None and (max_norm is not None or skip_nonfinite):
-                clip = _norm_and_factor(_List(what, lists[1]), math.inf if max_norm is None else max_norm)
-            rates = lr if isinstance(lr, (list, tuple)) else [lr] * n
-            for at in by_type.values():
-                _step(what, [[x[i] for i in at] for x in lists], moment_type, [rates[i] for i in at], betas, eps, [decay[i] for i in at], None,
-                      skip_nonfinite, clip, seed, at if ids is None else [ids[i] for i in at])
-            return None if clip is None else clip[0]
-        plain = T.step_lists(lists, moment_type, BLOCK)
-        if plain is None:
-            raise RuntimeError("%s: the lists changed while they were read" % what)
-    dtype, dev, ptrs, counts = plain
-    if extra or clip is not None:
-        for x in extra + ([] if clip is None else [clip]):
-            if x.get_device() != dev:
-                raise ValueError("%s: all tensors must be on one device (got cuda:%d and %s)" % (what, dev, x.device))
-    L = _lib.lib()
-    device = lists[0][0].device
+    for _, plain, _, _, tensors, _, _, _ in calls:
+        if tensors or clip is not None:
+            for x in tensors if clip is None else tensors + [clip]:
+                if x.get_device() != plain[1]:
+                    raise ValueError("%s: all tensors must be on one device (got cuda:%d and %s)" % (what, plain[1], x.device))
     limit = -1.0
-    if clip is None and (max_norm is not None or skip_nonfinite):    # the library computes the norm on its way
+    if clip is None and (max_norm is not None or skip_nonfinite):
         limit = math.inf if max_norm is None else max_norm
-        clip = torch.empty(2, dtype=torch.float32, device=device)
-    nbytes = L.dtt_adamw_workspace_bytes(n, counts)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    rates, decay = rates.tobytes(), decay.tobytes()
-    device_rates = None if device_rates is None else device_rates.tobytes()
-    tail = (beta1, beta2, eps, limit, None if clip is None else clip.data_ptr(), 1 if skip_nonfinite else 0, ws.data_ptr(), nbytes, _stream(dev))
-    with _on(dev):
-        if moment_type == 0:
-            p, g, s, m, v = ptrs
-            check(L.dtt_adamw_step(n, dtype, p, g, m, v, counts, s, rates, device_rates, decay, *tail), what)
-        else:
-            p, g, s, m, v, b = ptrs
-            ids = None if ids is None else array("I", [int(i) & 0xFFFFFFFF for i in ids]).tobytes()
-            check(L.dtt_adamw8_step(n, dtype, p, g, m, v, b, counts, s, rates, device_rates, decay, ids, int(seed) & 0xFFFFFFFF, *tail), what)
-    T.bump(lists[0])
+    if len(calls) > 1:
+        _check_together(what, calls, moment_type, clip)
+        if limit >= 0.0:                 # one norm over all of them
+            grads = _List(what, grads)
+            _device_of(what, [grads])
+            clip, limit = _norm_and_factor(grads, limit), -1.0
+    L, T = _lib.lib(), _tensorlist()
+    for lists, (dtype, dev, ptrs, counts), rates, device_rates, _, decay, (beta1, beta2, eps), ids in calls:
+        n, device = len(lists[0]), lists[0][0].device
+        if limit >= 0.0:                 # the library computes the norm on its way
+            clip = torch.empty(2, dtype=torch.float32, device=device)
+        nbytes = L.dtt_adamw_workspace_bytes(n, counts)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        rates, decay = rates.tobytes(), decay.tobytes()
+        device_rates = None if device_rates is None else device_rates.tobytes()
+        tail = (beta1, beta2, eps, limit, None if clip is None else clip.data_ptr(), 1 if skip_nonfinite else 0, ws.data_ptr(), nbytes, _stream(dev))
+        with _on(dev):
+            if moment_type == 0:
+                p, g, s, m, v = ptrs
+                check(L.dtt_adamw_step(n, dtype, p, g, m, v, counts, s, rates, device_rates, decay, *tail), what)
+            else:
+                p, g, s, m, v, b = ptrs
+                ids = None if ids is None else array("I", [int(i) & 0xFFFFFFFF for i in ids]).tobytes()
+                check(L.dtt_adamw8_step(n, dtype, p, g, m, v, b, counts, s, rates, device_rates, decay, ids, int(seed) & 0xFFFFFFFF, *tail), what)
+        T.bump(lists[0])
     return None if clip is None else clip[0]
 
 
@@ -312,8 +350,9 @@ def adamw_(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999
     2^-9 of its value.  lr and weight_decay: numbers, or a list with one for each tensor; lr also float32 tensors (read on the device).
     max_norm: c = min(1, max_norm / (norm + 1e-6)) of the norm over all gradients (which stay as they are), else c = 1.
     skip_nonfinite: where that norm is infinite or NaN, nothing changes, the counters neither.  clip: norm and factor computed before
-    (float32, 2 entries), in place of max_norm.  Returns the norm (float32 scalar on the device), or None without any of the three."""
-    return _step("adamw_", [params, grads, steps, exp_avgs, exp_avg_sqs], 0, lr, betas, eps, weight_decay, max_norm, skip_nonfinite, clip)
+    (float32, 2 entries), in place of max_norm.  Returns the norm (float32 scalar on the device), or None without any of the three.
+    Tensors of several types are one step: a call that is refused has changed nothing."""
+    return _step("adamw_", [([params, grads, steps, exp_avgs, exp_avg_sqs], lr, betas, eps, weight_decay, None)], 0, max_norm, skip_nonfinite, clip)
 
 
 def blocks_of(numel):
@@ -329,8 +368,8 @@ def adamw8_(params, grads, exp_avgs, exp_avg_sqs, bases, steps, *, lr, betas=(0.
     2^-15.7 below its block's largest is not moved.  The rounding of a moment is dithered, right on average, by a hash of seed, ids
     (default: the position in the list), step counter and element; the same inputs give the same codes.  Infinite and NaN moments stay
     in their element, as NaN."""
-    return _step("adamw8_", [params, grads, steps, exp_avgs, exp_avg_sqs, bases], _UINT8, lr, betas, eps, weight_decay, max_norm, skip_nonfinite,
-                 clip, seed, ids)
+    return _step("adamw8_", [([params, grads, steps, exp_avgs, exp_avg_sqs, bases], lr, betas, eps, weight_decay, ids)], _UINT8, max_norm,
+                 skip_nonfinite, clip, seed)
 
 
 def _check_bases(what, like, bases):
@@ -407,7 +446,8 @@ class GroupedAdamW(torch.optim.Optimizer):
     state_bits: 32, or 8 for uint8 moments (`exp_avg_code`, `exp_avg_sq_code`, `block_base`; see adamw8_); a checkpoint of either
     kind loads into the other.  max_norm: limit on the norm of all gradients, applied inside the step; the norm of the last step is
     `grad_norm` (float32 scalar on the device).  skip_nonfinite: a step whose gradients hold infinities or NaN changes nothing.
-    seed: of the rounding of 8-bit moments.  The moments of bfloat16 / float16 parameters are float32 too.
+    seed: of the rounding of 8-bit moments.  The moments of bfloat16 / float16 parameters are float32 too.  A step that is refused
+    has changed nothing, whatever its groups are.
 
     Before a step is captured into a graph it has to run once (the state is made at its first run), and the gradients have to keep
     their addresses.  amsgrad, maximize and the like are not offered."""
@@ -536,33 +576,34 @@ class GroupedAdamW(torch.optim.Optimizer):
         if not work:
             return loss
         what = "GroupedAdamW"
-        if fresh:       # (everything that would refuse the step does so before state is made)
+        if fresh:
             for rows in work.values():
                 p, g = _List(what, rows[0]).floats(what, "parameters").dense(what, "parameters"), _List(what, rows[1]).floats(what, "gradients")
                 _device_of(what, [p, g])
-            self._make_state(fresh)
-        limit, clip = self.max_norm, None
-        if (limit is not None or self.skip_nonfinite) and len(work) > 1:     # one norm over all of them
-            grads = _List(what, [g if _dense(g) else g.contiguous() for rows in work.values() for g in rows[1]]).floats(what, "gradients")
-            _device_of(what, [grads])
-            clip, limit = _norm_and_factor(grads, math.inf if limit is None else limit), None
-        norm = None
-        for (betas, eps), (params, grads, lr, decay, places) in work.items():
-            states = [state[p] for p in params]
-            m = [st[names[0]] for st in states]
-            at = _tensorlist().differ(params, m)
-            while at >= 0:      # the parameter took another memory order since (channels-last filters)
-                i = at >> 1
-                if at & 1 == 0:
-                    raise ValueError("GroupedAdamW: the state of a parameter of shape %s has shape %s" % (tuple(params[i].shape), tuple(m[i].shape)))
-                if torch.cuda.is_current_stream_capturing():
-                    raise RuntimeError("GroupedAdamW: run a step before capturing one (the state follows a parameter's new memory order)")
-                self._keep_moments(params[i], states[i], *self._moments(params[i], states[i]))
-                m[i] = states[i][names[0]]
+        try:
+            if fresh:
+                self._make_state(fresh)
+            jobs = []
+            for (betas, eps), (params, grads, lr, decay, places) in work.items():
+                states = [state[p] for p in params]
+                m = [st[names[0]] for st in states]
                 at = _tensorlist().differ(params, m)
-            lists = [params, grads, [st["step"] for st in states], m, [st[names[1]] for st in states]]
-            if self.state_bits == 8:
-                lists.append([st["block_base"] for st in states])
-            norm = _step(what, lists, 0 if self.state_bits == 32 else _UINT8, lr, betas, eps, decay, limit, self.skip_nonfinite, clip, self.seed, places)
-        self.grad_norm = norm
+                while at >= 0:      # the parameter took another memory order since (channels-last filters)
+                    i = at >> 1
+                    if at & 1 == 0:
+                        raise ValueError("GroupedAdamW: the state of a parameter of shape %s has shape %s" % (tuple(params[i].shape), tuple(m[i].shape)))
+                    if torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("GroupedAdamW: run a step before capturing one (the state follows a parameter's new memory order)")
+                    self._keep_moments(params[i], states[i], *self._moments(params[i], states[i]))
+                    m[i] = states[i][names[0]]
+                    at = _tensorlist().differ(params, m)
+                lists = [params, grads, [st["step"] for st in states], m, [st[names[1]] for st in states]]
+                if self.state_bits == 8:
+                    lists.append([st["block_base"] for st in states])
+                jobs.append((lists, lr, betas, eps, decay, places))
+            self.grad_norm = _step(what, jobs, 0 if self.state_bits == 32 else _UINT8, self.max_norm, self.skip_nonfinite, None, self.seed)
+        except Exception:
+            for p in fresh:         # a refused step leaves no state behind
+                state.pop(p, None)
+            raise
         return loss

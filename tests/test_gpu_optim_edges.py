@@ -1,0 +1,87 @@
+"""The optimizer operators (dtt/optim.py) where calls meet: lists of several types and groups of several betas as one step that is done or
+refused as a whole, versions, negated views, infinite limits."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+# ------------------------------------------------------------------------------------------------ refused as a whole
+def _mixed(bits, types=(torch.float32, torch.bfloat16, torch.float32), n=300):
+    """Lists of a step over several element types: [params, grads, m, v, (bases,) steps]."""
+    from dtt.optim import blocks_of
+    torch.manual_seed(1)
+    p = [torch.randn(n, device=DEV).to(t) for t in types]
+    g = [torch.randn_like(x) for x in p]
+    steps = [torch.zeros((), device=DEV) for _ in p]
+    if bits == 32:
+        return [p, g, [torch.zeros_like(x, dtype=torch.float32) for x in p], [torch.zeros_like(x, dtype=torch.float32) for x in p], steps]
+    return [p, g, [torch.zeros_like(x, dtype=torch.uint8) for x in p], [torch.zeros_like(x, dtype=torch.uint8) for x in p],
+            [torch.zeros(blocks_of(n), 2, dtype=torch.int16, device=DEV) for _ in p], steps]
+
+
+def _refused(lists, match, error=(ValueError, RuntimeError), **k):
+    from dtt.optim import adamw8_, adamw_
+    before = [[x.clone() for x in l] for l in lists]
+    with pytest.raises(error, match=match):
+        (adamw_ if len(lists) == 5 else adamw8_)(*lists, **dict(dict(lr=1e-2), **k))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for a, b in zip(lists, before) for x, y in zip(a, b)), "a refused step changed something"
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_step_over_several_types_is_refused_as_a_whole(bits):
+    lists = _mixed(bits)
+    lists[-1][1] = lists[-1][0]                                     # one counter for a float32 and a bfloat16 parameter
+    _refused(lists, "share memory")
+    lists = _mixed(bits)
+    lists[2][1] = lists[2][0]                                       # one moment
+    _refused(lists, "share memory")
+    lists = _mixed(bits)
+    lists[3][1] = lists[2][0]
+    _refused(lists, "share memory", max_norm=1.0)
+    lists = _mixed(bits, (torch.float16, torch.bfloat16, torch.float16))
+    lists[0][1] = lists[0][0].view(torch.bfloat16)                  # one parameter under two types
+    _refused(lists, "share memory")
+    lists = _mixed(bits)                                            # what only the second type's call would see
+    _refused(lists, "one device", lr=[torch.full((), 1e-2, device=DEV), torch.full((), 1e-2), 1e-2])
+    _refused(lists, "not be negative", weight_decay=[0.1, float("nan"), 0.1])
+    _refused(lists, "not be negative", lr=[0.1, float("nan"), 0.1], skip_nonfinite=True)
+    if bits == 8:
+        lists[4][1] = torch.zeros(5, dtype=torch.int16, device=DEV)[1:].view(2, 2)        # bases at an odd place
+        _refused(lists, "unaligned")
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_groups_of_different_betas_are_refused_as_a_whole(bits):
+    from dtt.optim import GroupedAdamW
+    torch.manual_seed(0)
+    ps = [torch.nn.Parameter(torch.randn(50, device=DEV)) for _ in range(3)]
+    opt = GroupedAdamW([{"params": [ps[0]]}, {"params": [ps[1]], "betas": (0.8, 0.9)}, {"params": [ps[2]], "eps": 1e-6}], lr=1e-2, state_bits=bits,
+                       max_norm=1.0)
+
+    def refused(match, error):
+        before = [p.detach().clone() for p in ps]
+        state = {i: {k: x.clone() for k, x in opt.state[p].items()} for i, p in enumerate(ps) if p in opt.state}
+        with pytest.raises(error, match=match):
+            opt.step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(ps, before))
+        assert {i for i, p in enumerate(ps) if opt.state.get(p)} == set(state)            # no state of a step that did not happen
+        assert all(torch.equal(x, opt.state[ps[i]][k]) for i, st in state.items() for k, x in st.items())
+    for p in ps:
+        p.grad = torch.randn_like(p)
+    opt.param_groups[1]["lr"] = -1.0
+    refused("lr must not be negative", ValueError)
+    opt.param_groups[1]["lr"] = 1e-2
+    opt.step()
+    opt.param_groups[2]["weight_decay"] = -1.0
+    refused("weight_decay must not be negative", ValueError)
+    opt.param_groups[2]["weight_decay"] = 0.0
+    own = opt.state[ps[2]]["step"]
+    opt.state[ps[2]]["step"] = opt.state[ps[0]]["step"]             # counted twice a step otherwise
+    refused("share memory", RuntimeError)
+    opt.state[ps[2]]["step"] = own
+    opt.step()
+    assert [float(opt.state[p]["step"]) for p in ps] == [2.0] * 3

@@ -34,3 +34,31 @@ def test_library_refuses_results_rates_and_workspaces_that_meet_a_tensor():
                         (dict(clip=base + 1026, limit=1.0), "unaligned"), (dict(w=m), "share memory"), (dict(w=base - 16), "share memory"),
                         (dict(rate=ws), "share memory")):
             assert step(bits, **kw) == 0 and why in _lib.last_error(), (bits, kw, _lib.last_error())
+
+
+def test_several_calls_are_checked_as_one_step():
+    """dtt_adamw_check: the tensors of all calls of a step, of whatever types, before the first is launched."""
+    from dtt import _lib
+    L = _lib.lib()
+    buf = (ctypes.c_double * 4096)()
+    base = ctypes.addressof(buf)
+    P = lambda *a: (ctypes.c_void_p * len(a))(*a)
+    N = lambda *a: (ctypes.c_long * len(a))(*a)
+    D = lambda *a: (ctypes.c_double * len(a))(*a)
+    I = lambda *a: (ctypes.c_int * len(a))(*a)
+
+    def together(dtypes=(0, 1), p=(base, base + 64), g=(base + 128, base + 192), m=(base + 256, base + 320), v=(base + 384, base + 448), b=None,
+                 n=(16, 16), s=(base + 512, base + 516), lr=(1e-3, 1e-3), rate=None, wd=(0.0, 0.0), clip=None):
+        return L.dtt_adamw_check(2, I(*dtypes), P(*p), P(*g), P(*m), P(*v), None if b is None else P(*b), N(*n), P(*s), D(*lr),
+                                 None if rate is None else P(*rate), D(*wd), clip)
+    bases = (base + 600, base + 604)
+    assert together() == 1 and together(b=bases) == 1 and together(n=(0, 16), p=(None, base + 64), clip=base + 1024, rate=(base + 1100, None)) == 1
+    assert together(m=(base + 256, base + 280), b=bases) == 1      # 16 codes are 16 bytes; 16 values are 64
+    for kw, why in ((dict(s=(base + 512, base + 512)), "share memory"), (dict(m=(base + 256, base + 280)), "share memory"),
+                    (dict(p=(base, base + 60)), "share memory"), (dict(g=(base + 128, base + 60)), "share memory"),
+                    (dict(b=(base + 600, base + 600)), "share memory"), (dict(b=(base + 600, base + 606)), "unaligned"), (dict(b=(base + 600, None)), "null"),
+                    (dict(v=(base + 384, base + 450)), "unaligned"), (dict(p=(base, base + 65)), "unaligned"), (dict(dtypes=(0, 3)), "element type"),
+                    (dict(n=(16, -1)), "element count"), (dict(lr=(1e-3, float("nan"))), "learning rate"), (dict(wd=(0.0, -1.0)), "weight decay"),
+                    (dict(rate=(None, base + 68)), "share memory"), (dict(clip=base + 512), "share memory"), (dict(s=(base + 512, None)), "step counter")):
+        assert together(**kw) == 0 and why in _lib.last_error(), (kw, _lib.last_error())
+    assert L.dtt_adamw_check(0, None, *[None] * 11) == 1
