@@ -25,6 +25,8 @@ _UINT8 = 3
 BLOCK = 256                      # elements, in memory order, that share a base of the 8-bit moments
 _NAN_FLAG = 0x4000
 _ONE = (1).to_bytes(8, "little")
+_MOMENTS32 = ("exp_avg", "exp_avg_sq")                               # entries of the optimizer's state
+_MOMENTS8 = ("exp_avg_code", "exp_avg_sq_code", "block_base")
 
 _host = None
 
@@ -507,40 +509,49 @@ class GroupedAdamW(torch.optim.Optimizer):
     def _keep_moments(self, p, st, m, v):
         """The state entries for float32 moments, in the parameter's memory order and this optimizer's form."""
         m, v = (torch.empty_like(p, dtype=torch.float32).copy_(x) for x in (m, v))
-        for k in ("exp_avg", "exp_avg_sq", "exp_avg_code", "exp_avg_sq_code", "block_base"):
+        for k in _MOMENTS32 + _MOMENTS8:
             st.pop(k, None)
         if self.state_bits == 32:
             st["exp_avg"], st["exp_avg_sq"] = m, v
         else:
             st["exp_avg_code"], st["exp_avg_sq_code"], st["block_base"] = pack_moments(m, v)
 
+    def _saved(self, src, p):
+        """The names of a parameter's moments in a checkpoint; raises where the entry is not a state of this parameter."""
+        if "step" not in src or not any(all(k in src for k in names) for names in (_MOMENTS32, _MOMENTS8)):
+            raise ValueError("GroupedAdamW: not a state of AdamW or Adam (it holds %s)" % sorted(src))
+        if torch.as_tensor(src["step"]).numel() != 1:
+            raise ValueError("GroupedAdamW: step is one number (the checkpoint has shape %s)" % (tuple(src["step"].shape),))
+        names = _MOMENTS32 if all(k in src for k in _MOMENTS32) else _MOMENTS8
+        if names is _MOMENTS8 and self.state_bits == 32 and not p.is_cuda:
+            raise RuntimeError("dtt ops run on the GPU only (8-bit moments of a parameter on %s); there is no CPU fallback" % p.device)
+        return names
+
     @torch.no_grad()
     def load_state_dict(self, state_dict):
         """Of this class (32 or 8 bits) or of torch.optim.AdamW / Adam.  The moments keep float32 (or their codes) whatever the
-        parameters' type is, and are re-packed where the other form was saved."""
+        parameters' type is, and are re-packed where the other form was saved.  A checkpoint that is refused changes nothing."""
         for g in state_dict["param_groups"]:
             if g.get("amsgrad") or g.get("maximize"):
                 raise ValueError("GroupedAdamW: a checkpoint with amsgrad or maximize does not load")
-        saved = dict(state_dict["state"])
-        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
+        names = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        saved = [(p, state_dict["state"][i]) for i, p in zip(names, params) if i in state_dict["state"]]
+        saved = [(p, src, self._saved(src, p)) for p, src in saved]
+        for g in state_dict["param_groups"]:
+            missing = [k for k in ("lr", "betas", "eps", "weight_decay") if k not in g]
+            if missing:
+                raise ValueError("GroupedAdamW: not a checkpoint of AdamW or Adam (a group without %s)" % ", ".join(missing))
+        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})   # (refuses groups of other sizes first)
         for g in self.param_groups:
             if isinstance(g["lr"], torch.Tensor) and g["params"]:   # (a checkpoint read into host memory)
                 g["lr"] = g["lr"].to(device=g["params"][0].device, dtype=torch.float32)
-        names = [i for g in state_dict["param_groups"] for i in g["params"]]
-        for i, p in zip(names, [p for g in self.param_groups for p in g["params"]]):
-            if i not in saved:
-                continue
-            src = saved[i]
-            if "step" not in src or not ("exp_avg" in src or "exp_avg_code" in src):
-                raise ValueError("GroupedAdamW: not a state of AdamW or Adam (it holds %s)" % sorted(src))
+        for p, src, moments in saved:
             st = self.state[p]
-            t = src["step"]
-            st["step"] = torch.as_tensor(t).detach().clone().to(device=p.device, dtype=torch.float32).reshape(())
-            for k, dt in (("exp_avg", torch.float32), ("exp_avg_sq", torch.float32), ("exp_avg_code", torch.uint8),
-                          ("exp_avg_sq_code", torch.uint8), ("block_base", torch.int16)):
-                if k in src:
-                    st[k] = src[k].detach().to(device=p.device, dtype=dt, copy=True)
-            if ("exp_avg" in st) != (self.state_bits == 32):
+            st["step"] = torch.as_tensor(src["step"]).detach().clone().to(device=p.device, dtype=torch.float32).reshape(())
+            for k, dt in zip(moments, (torch.float32, torch.float32) if moments is _MOMENTS32 else (torch.uint8, torch.uint8, torch.int16)):
+                st[k] = src[k].detach().to(device=p.device, dtype=dt, copy=True)
+            if (moments is _MOMENTS32) != (self.state_bits == 32):
                 self._keep_moments(p, st, *self._moments(p, st))
 
     # ------------------------------------------------------------------ step
@@ -552,7 +563,7 @@ class GroupedAdamW(torch.optim.Optimizer):
                 loss = closure()
         work, fresh = {}, []
         state, place = self.state, -1
-        names = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("exp_avg_code", "exp_avg_sq_code")
+        names = _MOMENTS32 if self.state_bits == 32 else _MOMENTS8
         for g in self.param_groups:
             key = (g["betas"], g["eps"])
             key = key if type(key[0]) is tuple else (tuple(key[0]), key[1])

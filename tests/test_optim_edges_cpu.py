@@ -1,8 +1,10 @@
 """The optimizer operators where calls meet, without a GPU: what the library refuses about buffers that meet, checkpoints that are refused,
 learning rates that groups share."""
+import copy
 import ctypes
 
 import pytest
+import torch
 
 
 def test_library_refuses_results_rates_and_workspaces_that_meet_a_tensor():
@@ -62,3 +64,54 @@ def test_several_calls_are_checked_as_one_step():
                     (dict(rate=(None, base + 68)), "share memory"), (dict(clip=base + 512), "share memory"), (dict(s=(base + 512, None)), "step counter")):
         assert together(**kw) == 0 and why in _lib.last_error(), (kw, _lib.last_error())
     assert L.dtt_adamw_check(0, None, *[None] * 11) == 1
+
+
+def _adamw_state(shape=(4, 3), step=3.0):
+    torch.manual_seed(0)
+    return {"step": torch.tensor(step), "exp_avg": torch.randn(shape), "exp_avg_sq": torch.rand(shape)}
+
+
+def _optimizer(bits=32):
+    """Two parameters of an optimizer that holds a state (read from a checkpoint: 32-bit moments need no GPU)."""
+    from dtt.optim import GroupedAdamW
+    ps = [torch.nn.Parameter(torch.ones(4, 3)) for _ in range(2)]
+    opt = GroupedAdamW([{"params": [ps[0]], "lr": 0.5}, {"params": [ps[1]], "betas": (0.8, 0.9)}], lr=0.25, state_bits=bits)
+    sd = opt.state_dict()
+    sd["state"] = {0: _adamw_state(), 1: _adamw_state(step=7.0)}
+    opt.load_state_dict(sd)
+    return opt, ps
+
+
+def _refused_load(opt, ps, checkpoint, match):
+    groups = copy.deepcopy([{k: v for k, v in g.items() if k != "params"} for g in opt.param_groups])
+    state = [{k: x.clone() for k, x in opt.state[p].items()} for p in ps]
+    with pytest.raises(ValueError, match=match):
+        opt.load_state_dict(checkpoint)
+    assert [{k: v for k, v in g.items() if k != "params"} for g in opt.param_groups] == groups
+    assert [g["params"][0] is p for g, p in zip(opt.param_groups, ps)] == [True, True]
+    assert len(opt.state) == 2
+    for p, st in zip(ps, state):
+        assert set(opt.state[p]) == set(st) and all(torch.equal(opt.state[p][k], x) for k, x in st.items())
+
+
+def test_a_refused_checkpoint_leaves_the_optimizer_as_it_was():
+    for bits in (32, 8):
+        opt, ps = _optimizer(bits)
+        sgd = torch.optim.SGD([{"params": [p]} for p in ps], lr=0.1, momentum=0.9)
+        for p in ps:
+            p.grad = torch.ones_like(p)
+        sgd.step()
+        _refused_load(opt, ps, sgd.state_dict(), "not a state of AdamW")
+        plain = torch.optim.SGD([{"params": [p]} for p in ps], lr=0.1).state_dict()        # its groups have no betas, and there is no state to tell
+        _refused_load(opt, ps, plain, "betas")
+        good = lambda: copy.deepcopy(opt.state_dict())
+        for change, why in ((lambda d: d["param_groups"][1].update(amsgrad=True), "amsgrad"),
+                            (lambda d: d["state"][1].pop("step"), "not a state of AdamW"),
+                            (lambda d: d["state"][1].pop("exp_avg_sq" if bits == 32 else "exp_avg_sq_code"), "not a state of AdamW"),
+                            (lambda d: d["param_groups"].pop(), "parameter group"),
+                            (lambda d: d["param_groups"][1]["params"].append(2), "parameter group"),
+                            (lambda d: d["state"][1].update(step=torch.zeros(2)), "step")):
+            d = good()
+            change(d)
+            _refused_load(opt, ps, d, why)
+        opt.load_state_dict(good())
