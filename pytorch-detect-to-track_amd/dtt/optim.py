@@ -508,6 +508,8 @@ class GroupedAdamW(torch.optim.Optimizer):
 
     def _keep_moments(self, p, st, m, v):
         """The state entries for float32 moments, in the parameter's memory order and this optimizer's form."""
+        if m.shape != p.shape or v.shape != p.shape:
+            raise ValueError("GroupedAdamW: the state of a parameter of shape %s has shapes %s and %s" % (tuple(p.shape), tuple(m.shape), tuple(v.shape)))
         m, v = (torch.empty_like(p, dtype=torch.float32).copy_(x) for x in (m, v))
         for k in _MOMENTS32 + _MOMENTS8:
             st.pop(k, None)
@@ -523,6 +525,15 @@ class GroupedAdamW(torch.optim.Optimizer):
         if torch.as_tensor(src["step"]).numel() != 1:
             raise ValueError("GroupedAdamW: step is one number (the checkpoint has shape %s)" % (tuple(src["step"].shape),))
         names = _MOMENTS32 if all(k in src for k in _MOMENTS32) else _MOMENTS8
+        m, v = (src[k] for k in names[:2])
+        if m.shape != p.shape or v.shape != p.shape:
+            raise ValueError("GroupedAdamW: moments have their parameter's shape (the checkpoint has %s and %s for %s)" %
+                             (tuple(m.shape), tuple(v.shape), tuple(p.shape)))
+        if names is _MOMENTS8:
+            if m.dtype != torch.uint8 or v.dtype != torch.uint8 or not _dense(m) or not _same_order(m, v):
+                raise ValueError("GroupedAdamW: codes are uint8, dense, both in one memory order (the checkpoint has %s, strides %s and %s, strides %s)" %
+                                 (m.dtype, m.stride(), v.dtype, v.stride()))
+            _check_bases("GroupedAdamW", [m], [src[names[2]]])
         if names is _MOMENTS8 and self.state_bits == 32 and not p.is_cuda:
             raise RuntimeError("dtt ops run on the GPU only (8-bit moments of a parameter on %s); there is no CPU fallback" % p.device)
         return names
@@ -551,7 +562,7 @@ class GroupedAdamW(torch.optim.Optimizer):
             st["step"] = torch.as_tensor(src["step"]).detach().clone().to(device=p.device, dtype=torch.float32).reshape(())
             for k, dt in zip(moments, (torch.float32, torch.float32) if moments is _MOMENTS32 else (torch.uint8, torch.uint8, torch.int16)):
                 st[k] = src[k].detach().to(device=p.device, dtype=dt, copy=True)
-            if (moments is _MOMENTS32) != (self.state_bits == 32):
+            if (moments is _MOMENTS32) != (self.state_bits == 32) or not _same_order(st[moments[0]], st[moments[1]]):
                 self._keep_moments(p, st, *self._moments(p, st))
 
     # ------------------------------------------------------------------ step

@@ -115,3 +115,41 @@ def test_a_refused_checkpoint_leaves_the_optimizer_as_it_was():
             change(d)
             _refused_load(opt, ps, d, why)
         opt.load_state_dict(good())
+
+
+def test_moments_of_another_shape_do_not_load():
+    """A state of another shape would be broadcast into the parameter's, or refused at the next step only."""
+    from dtt.optim import pack_moments
+    for bits in (32, 8):
+        opt, ps = _optimizer(bits)
+        with32 = lambda: {"param_groups": copy.deepcopy(opt.state_dict()["param_groups"]), "state": {0: _adamw_state(), 1: _adamw_state()}}
+
+        def with8():
+            d = with32()
+            for i in d["state"]:
+                st = d["state"][i]
+                st["exp_avg_code"], st["exp_avg_sq_code"], st["block_base"] = pack_moments(st.pop("exp_avg"), st.pop("exp_avg_sq"))
+            return d
+        for shape in ((3,), (1,), (), (4, 1), (3, 4), (12,), (4, 4)):
+            for k in ("exp_avg", "exp_avg_sq"):
+                d = with32()
+                d["state"][1][k] = torch.ones(shape)
+                _refused_load(opt, ps, d, "shape")
+        if bits == 8:
+            for change in (lambda st: st.update(exp_avg_code=st["exp_avg_code"][0]), lambda st: st.update(exp_avg_sq_code=st["exp_avg_sq_code"].view(3, 4)),
+                           lambda st: st.update(exp_avg_code=st["exp_avg_code"].t().contiguous().t()),            # the two lie in other orders
+                           lambda st: st.update(exp_avg_code=torch.zeros(4, 6, dtype=torch.uint8)[:, ::2], exp_avg_sq_code=torch.zeros(4, 6, dtype=torch.uint8)[:, ::2]),
+                           lambda st: st.update(exp_avg_code=st["exp_avg_code"].int()), lambda st: st.update(block_base=torch.zeros(2, 2, dtype=torch.int16)),
+                           lambda st: st.update(block_base=torch.zeros(1, 2, dtype=torch.int32))):
+                d = with8()
+                change(d["state"][1])
+                _refused_load(opt, ps, d, "shape|int16|uint8")
+            opt.load_state_dict(with8())
+        opt.load_state_dict(with32())
+    opt, ps = _optimizer()
+    d = opt.state_dict()
+    d["state"] = {0: _adamw_state(), 1: _adamw_state()}
+    d["state"][0]["exp_avg_sq"] = d["state"][0]["exp_avg_sq"].t().contiguous().t()         # the same values in another memory order do
+    want = d["state"][0]["exp_avg_sq"].clone()
+    opt.load_state_dict(d)
+    assert opt.state[ps[0]]["exp_avg_sq"].is_contiguous() and torch.equal(opt.state[ps[0]]["exp_avg_sq"], want)
