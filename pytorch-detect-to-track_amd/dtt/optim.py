@@ -554,9 +554,13 @@ class GroupedAdamW(torch.optim.Optimizer):
             if missing:
                 raise ValueError("GroupedAdamW: not a checkpoint of AdamW or Adam (a group without %s)" % ", ".join(missing))
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})   # (refuses groups of other sizes first)
+        moved = {}          # a rate that groups share stays one tensor
         for g in self.param_groups:
             if isinstance(g["lr"], torch.Tensor) and g["params"]:   # (a checkpoint read into host memory)
-                g["lr"] = g["lr"].to(device=g["params"][0].device, dtype=torch.float32)
+                lr, dev = g["lr"], g["params"][0].device
+                if (id(lr), dev) not in moved:
+                    moved[id(lr), dev] = lr, lr.to(device=dev, dtype=torch.float32)
+                g["lr"] = moved[id(lr), dev][1]
         for p, src, moments in saved:
             st = self.state[p]
             st["step"] = torch.as_tensor(src["step"]).detach().clone().to(device=p.device, dtype=torch.float32).reshape(())

@@ -153,3 +153,20 @@ def test_moments_of_another_shape_do_not_load():
     want = d["state"][0]["exp_avg_sq"].clone()
     opt.load_state_dict(d)
     assert opt.state[ps[0]]["exp_avg_sq"].is_contiguous() and torch.equal(opt.state[ps[0]]["exp_avg_sq"], want)
+
+
+def test_groups_that_share_a_learning_rate_share_it_after_a_checkpoint():
+    """One rate tensor for all groups (what a schedule under a graph writes to) stays one, also where it is converted."""
+    from dtt.optim import GroupedAdamW
+    for dtype in (torch.float32, torch.float64):
+        ps = [torch.nn.Parameter(torch.ones(3)) for _ in range(4)]
+        rate, other = torch.tensor(0.25, dtype=dtype), torch.tensor(0.5, dtype=dtype)
+        groups = lambda: [{"params": [p], "lr": r} for p, r in zip(ps, (rate, rate, other, rate))]
+        saved = torch.optim.AdamW(groups(), lr=0.1, foreach=False, capturable=True).state_dict()
+        opt = GroupedAdamW([{"params": [p]} for p in ps], lr=0.125)
+        opt.load_state_dict(saved)
+        lr = [g["lr"] for g in opt.param_groups]
+        assert all(x.dtype == torch.float32 for x in lr) and [float(x) for x in lr] == [0.25, 0.25, 0.5, 0.25]
+        assert lr[0] is lr[1] and lr[0] is lr[3] and lr[2] is not lr[0]
+        lr[0].fill_(1.0)
+        assert [float(g["lr"]) for g in opt.param_groups] == [1.0, 1.0, 0.5, 1.0] and float(rate) == 0.25
