@@ -600,6 +600,7 @@ class GroupedAdamW(torch.optim.Optimizer):
                 rows[4].append(place)
         work = {k: rows for k, rows in work.items() if rows[0]}
         if not work:
+            self.grad_norm = None
             return loss
         what = "GroupedAdamW"
         if fresh:

@@ -170,3 +170,12 @@ def test_groups_that_share_a_learning_rate_share_it_after_a_checkpoint():
         assert lr[0] is lr[1] and lr[0] is lr[3] and lr[2] is not lr[0]
         lr[0].fill_(1.0)
         assert [float(g["lr"]) for g in opt.param_groups] == [1.0, 1.0, 0.5, 1.0] and float(rate) == 0.25
+
+
+def test_a_step_without_gradients_has_no_norm():
+    from dtt.optim import GroupedAdamW
+    p = torch.nn.Parameter(torch.ones(3))
+    opt = GroupedAdamW([p], max_norm=1.0)
+    opt.grad_norm = torch.ones(())                  # of the step before
+    opt.step()
+    assert opt.grad_norm is None
