@@ -104,7 +104,7 @@ def _limit(what, max_norm):
 
 
 def _written(*lists):
-    """The kernels write behind autograd's back: tell it, as torch's own in-place operations do."""
+    """The kernels write behind autograd's back: tell it of these tensors, as torch's own in-place operations do."""
     _tensorlist().bump(*lists)
 
 
@@ -152,7 +152,8 @@ def grad_norm(grads):
 def clip_grads_(grads, max_norm):
     """Scale all gradients in place by min(1, max_norm / (norm + 1e-6)) and return their norm before that (float32 scalar on their
     device).  Gradients within the limit are not written.  Mixed float32 / bfloat16 / float16 tensors are one vector.  An infinite norm
-    gives the factor 0 and NaN gives NaN, as the formula has it; no tensor may appear twice."""
+    gives the factor 0 and NaN gives NaN, as the formula has it; an infinite limit asks for the norm alone and leaves the gradients as they
+    are, whatever it is.  No tensor may appear twice."""
     max_norm = _limit("clip_grads_", max_norm)
     grads = _gradients("clip_grads_", grads)
     if not len(grads):
@@ -338,7 +339,7 @@ def _step(what, jobs, moment_type, max_norm, skip_nonfinite, clip, seed=0):
                 p, g, s, m, v, b = ptrs
                 ids = None if ids is None else array("I", [int(i) & 0xFFFFFFFF for i in ids]).tobytes()
                 check(L.dtt_adamw8_step(n, dtype, p, g, m, v, b, counts, s, rates, device_rates, decay, ids, int(seed) & 0xFFFFFFFF, *tail), what)
-        T.bump(lists[0])
+        T.bump(lists[0])     # (the state is the optimizer's own: its versions would cost 18 us of a 75 us step of 301 tensors)
     return None if clip is None else clip[0]
 
 
@@ -353,7 +354,8 @@ def adamw_(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999
     max_norm: c = min(1, max_norm / (norm + 1e-6)) of the norm over all gradients (which stay as they are), else c = 1.
     skip_nonfinite: where that norm is infinite or NaN, nothing changes, the counters neither.  clip: norm and factor computed before
     (float32, 2 entries), in place of max_norm.  Returns the norm (float32 scalar on the device), or None without any of the three.
-    Tensors of several types are one step: a call that is refused has changed nothing."""
+    Tensors of several types are one step: a call that is refused has changed nothing.  Autograd is told that the parameters changed;
+    moments and counters do not count a version."""
     return _step("adamw_", [([params, grads, steps, exp_avgs, exp_avg_sqs], lr, betas, eps, weight_decay, None)], 0, max_norm, skip_nonfinite, clip)
 
 

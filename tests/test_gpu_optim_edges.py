@@ -1,5 +1,7 @@
 """The optimizer operators (dtt/optim.py) where calls meet: lists of several types and groups of several betas as one step that is done or
-refused as a whole, versions, negated views, infinite limits."""
+refused as a whole, infinite limits."""
+import math
+
 import pytest
 import torch
 
@@ -85,3 +87,19 @@ def test_groups_of_different_betas_are_refused_as_a_whole(bits):
     opt.state[ps[2]]["step"] = own
     opt.step()
     assert [float(opt.state[p]["step"]) for p in ps] == [2.0] * 3
+
+
+# ------------------------------------------------------------------------------------------------ limits
+def test_an_infinite_limit_leaves_the_gradients_whatever_their_norm():
+    from dtt.optim import clip_grads_
+    for odd in (math.nan, math.inf):
+        g = torch.ones(1000, device=DEV)
+        g[7] = odd
+        want = g.clone()
+        norm = float(clip_grads_([g], math.inf))
+        assert math.isnan(norm) if math.isnan(odd) else math.isinf(norm)
+        assert torch.equal(g.isnan(), want.isnan()) and torch.equal(g.nan_to_num(), want.nan_to_num())
+    g = torch.ones(1000, device=DEV)
+    g[7] = math.nan
+    clip_grads_([g], 1.0)                                           # a finite limit: the factor is NaN as the norm is
+    assert bool(g.isnan().all())
