@@ -15,7 +15,7 @@ enum { kOther = -1, kF32 = 0, kBf16 = 1, kF16 = 2, kU8 = 3, kI16 = 4 };
 enum { kNone = -3, kSeveral = -2, kHost = -1 };   // devices beside an index
 
 int type_code(const at::Tensor& t) {
-  if (t.layout() != at::kStrided) return kOther;
+  if (t.layout() != at::kStrided || t.is_neg()) return kOther;   // (a negated view's memory is not its values)
   switch (t.scalar_type()) {
     case at::kFloat: return kF32;
     case at::kBFloat16: return kBf16;

@@ -63,8 +63,8 @@ class _List:
         """All strided float32, bfloat16 or float16."""
         if not 0 <= self.type <= 2:
             for t in self.tensors:
-                if t.layout != torch.strided or t.dtype not in _DTYPES:
-                    raise TypeError("%s: %s must be dense float32, bfloat16 or float16 tensors (got %s, %s)" % (what, name, t.dtype, t.layout))
+                if t.layout != torch.strided or t.dtype not in _DTYPES or t.is_neg():
+                    raise TypeError("%s: %s must be dense float32, bfloat16 or float16 tensors (got %s, %s)" % (what, name, _kind(t), t.layout))
         return self
 
     def dense(self, what, name):
@@ -72,6 +72,11 @@ class _List:
             t = self.tensors[self.odd]
             raise ValueError("%s: %s must be dense (entry %d: shape %s, strides %s)" % (what, name, self.odd, tuple(t.shape), t.stride()))
         return self
+
+
+def _kind(t):
+    """A tensor's type, and what keeps its memory from being its values."""
+    return "%s%s" % (t.dtype, ", a negated view: resolve_neg() first" if t.is_neg() else "")
 
 
 def _device_of(what, lists):
@@ -166,15 +171,15 @@ def clip_grads_(grads, max_norm):
 @torch.no_grad()
 def clip_grad_norm_(parameters, max_norm):
     """torch.nn.utils.clip_grad_norm_ (2-norm) in a few launches: clip_grads_ over the gradients of `parameters` (a tensor or an
-    iterable; those without a gradient are left out, a gradient that is an expanded view is made dense first)."""
+    iterable; those without a gradient are left out, a gradient that is an expanded or negated view is made dense first)."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     grads = []
     for p in parameters:
         g = p.grad
         if g is None:
             continue
-        if g.layout == torch.strided and not _dense(g):
-            g = p.grad = g.detach().contiguous()
+        if g.layout == torch.strided and (g.is_neg() or not _dense(g)):
+            g = p.grad = g.detach().resolve_neg().contiguous()
         grads.append(g)
     return clip_grads_(grads, max_norm)
 
@@ -202,8 +207,8 @@ def _rates(what, lr, n):
         return _numbers(what, "lr", lr, n), None, []
     tensors = [x for x in lr if isinstance(x, torch.Tensor)]
     for x in tensors:
-        if x.numel() != 1 or x.dtype != torch.float32:
-            raise TypeError("%s: a learning rate in device memory is one float32 (got %s, %s)" % (what, tuple(x.shape), x.dtype))
+        if x.numel() != 1 or x.dtype != torch.float32 or x.is_neg():
+            raise TypeError("%s: a learning rate in device memory is one float32 (got %s, %s)" % (what, tuple(x.shape), _kind(x)))
     return (_numbers(what, "lr", [0.0 if isinstance(x, torch.Tensor) else x for x in lr], n),
             array("Q", [x.data_ptr() if isinstance(x, torch.Tensor) else 0 for x in lr]), tensors)
 
@@ -212,6 +217,9 @@ def _mend(what, lists, moment_type):
     """Why the lists of a step are not plain: raises what is wrong with them, or returns them with gradients in their parameters' order."""
     params, grads, steps = lists[:3]
     p, g, s = (_List(what, x) for x in lists[:3])
+    if g.types != p.types:
+        grads = [y.resolve_neg() if y.layout == torch.strided else y for y in grads]
+        g = _List(what, grads)
     p.floats(what, "parameters").dense(what, "parameters")
     if g.types != p.types:
         raise TypeError("%s: a gradient has its parameter's type (got %s for %s)" % ((what,) + next(
@@ -220,13 +228,13 @@ def _mend(what, lists, moment_type):
         if x.shape != y.shape:
             raise ValueError("%s: a gradient has its parameter's shape (got %s for %s)" % (what, tuple(y.shape), tuple(x.shape)))
     if s.type != 0 or s.counts != _ONE * len(steps):
-        bad = next(t for t in steps if t.dtype != torch.float32 or t.numel() != 1 or t.layout != torch.strided)
-        raise TypeError("%s: a step counter is one float32 (got %s, %s)" % (what, tuple(bad.shape), bad.dtype))
+        bad = next(t for t in steps if t.dtype != torch.float32 or t.numel() != 1 or t.layout != torch.strided or t.is_neg())
+        raise TypeError("%s: a step counter is one float32 (got %s, %s)" % (what, tuple(bad.shape), _kind(bad)))
     _device_of(what, [p, g, s] + [_List(what, x) for x in lists[3:]])
     for x in lists[3:5]:
         m = _List(what, x)
         if m.type != moment_type:
-            raise TypeError("%s: moments must be %s (got %s)" % (what, "float32" if moment_type == 0 else "uint8", sorted({str(t.dtype) for t in x})))
+            raise TypeError("%s: moments must be %s (got %s)" % (what, "float32" if moment_type == 0 else "uint8", sorted({_kind(t) for t in x})))
         at = _tensorlist().differ(params, x)
         if at >= 0:
             t, q = x[at >> 1], params[at >> 1]
@@ -298,7 +306,7 @@ def _step(what, jobs, moment_type, max_norm, skip_nonfinite, clip, seed=0):
     whole.  Returns the norm or None."""
     if max_norm is not None:
         max_norm = _limit(what, max_norm)
-    if clip is not None and (max_norm is not None or clip.dtype != torch.float32 or tuple(clip.shape) != (2,) or not clip.is_contiguous()):
+    if clip is not None and (max_norm is not None or clip.dtype != torch.float32 or tuple(clip.shape) != (2,) or not clip.is_contiguous() or clip.is_neg()):
         raise ValueError("%s: clip is norm and factor, two float32, and stands in place of max_norm" % what)
     calls, grads = [], []
     for job in jobs:
@@ -607,8 +615,7 @@ class GroupedAdamW(torch.optim.Optimizer):
         what = "GroupedAdamW"
         if fresh:
             for rows in work.values():
-                p, g = _List(what, rows[0]).floats(what, "parameters").dense(what, "parameters"), _List(what, rows[1]).floats(what, "gradients")
-                _device_of(what, [p, g])
+                _device_of(what, [_List(what, rows[0]).floats(what, "parameters").dense(what, "parameters"), _List(what, rows[1])])
         try:
             if fresh:
                 self._make_state(fresh)

@@ -103,3 +103,41 @@ def test_an_infinite_limit_leaves_the_gradients_whatever_their_norm():
     g[7] = math.nan
     clip_grads_([g], 1.0)                                           # a finite limit: the factor is NaN as the norm is
     assert bool(g.isnan().all())
+
+
+# ------------------------------------------------------------------------------------------------ negated views
+def test_negated_views_are_read_as_what_they_are_or_refused():
+    from dtt.optim import GroupedAdamW, adamw_, clip_grad_norm_, clip_grads_, grad_norm
+    g = torch.randn(100, device=DEV)
+    neg = torch._neg_view(g)
+    assert neg.is_neg()
+    p, q = torch.zeros(100, device=DEV), torch.zeros(100, device=DEV)
+    state = lambda: ([torch.zeros(100, device=DEV)], [torch.zeros(100, device=DEV)], [torch.zeros((), device=DEV)])
+    adamw_([p], [neg], *state(), lr=0.1)
+    adamw_([q], [-g], *state(), lr=0.1)
+    assert torch.equal(p, q) and p.any()
+    with pytest.raises(TypeError, match="resolve_neg"):
+        clip_grads_([neg], 0.1)
+    with pytest.raises(TypeError, match="resolve_neg"):
+        adamw_([torch._neg_view(p)], [g], *state(), lr=0.1)
+    m, v, s = state()
+    with pytest.raises(TypeError, match="resolve_neg"):
+        adamw_([p], [g], [torch._neg_view(m[0])], v, s, lr=0.1)
+    with pytest.raises(TypeError, match="resolve_neg"):
+        adamw_([p], [g], m, v, [torch._neg_view(s[0])], lr=0.1)
+    with pytest.raises(TypeError, match="resolve_neg"):
+        grad_norm([neg])
+    w, u = torch.nn.Parameter(torch.zeros(100, device=DEV)), torch.nn.Parameter(torch.zeros(100, device=DEV))
+    w.grad, u.grad = torch._neg_view(g.clone()), -g
+    a, b = clip_grad_norm_([w], 0.5), clip_grad_norm_([u], 0.5)
+    assert torch.equal(a, b) and torch.equal(w.grad, u.grad)
+    w.grad, u.grad = torch._neg_view(g.clone()), -g
+    for x in (w, u):
+        GroupedAdamW([x], lr=0.1, max_norm=1.0).step()
+    assert torch.equal(w, u)
+    w2, w3 = torch.nn.Parameter(w.detach().clone()), torch.nn.Parameter(w.detach().clone())
+    u2, u3 = torch.nn.Parameter(w.detach().clone()), torch.nn.Parameter(w.detach().clone())
+    for x, y in ((w2, w3), (u2, u3)):                               # two betas: one norm over both
+        x.grad, y.grad = (torch._neg_view(g.clone()), g.clone()) if x is w2 else (-g, g.clone())
+        GroupedAdamW([{"params": [x]}, {"params": [y], "betas": (0.8, 0.9)}], lr=0.1, max_norm=1.0).step()
+    assert torch.equal(w2, u2) and torch.equal(w3, u3)

@@ -179,3 +179,20 @@ def test_a_step_without_gradients_has_no_norm():
     opt.grad_norm = torch.ones(())                  # of the step before
     opt.step()
     assert opt.grad_norm is None
+
+
+def test_a_negated_view_is_not_its_memory():
+    """The imaginary part of a conjugate: float32, strided, and the negative of what lies in memory."""
+    from dtt import optim as O
+    z = torch.complex(torch.ones(1), torch.full((1,), 2.0)).conj()
+    g = z.imag
+    assert g.is_neg() and float(g) == -2.0
+    p, m, v, s = torch.zeros(1), torch.zeros(1), torch.zeros(1), torch.zeros(())
+    for call in (lambda: O.grad_norm([g]), lambda: O.clip_grads_([g], 1.0), lambda: O.adamw_([g], [p], [m], [v], [s], lr=0.1),
+                 lambda: O.adamw_([p], [m], [g], [v], [s], lr=0.1), lambda: O.adamw_([p], [m], [v], [s], [g.view(())], lr=0.1),
+                 lambda: O.adamw_([p], [m], [v], [torch.zeros(1)], [s], lr=g)):
+        with pytest.raises((TypeError, RuntimeError), match="resolve_neg|GPU only"):
+            call()
+    assert O._tensorlist().describe([g])[4] == -1
+    with pytest.raises(TypeError, match="resolve_neg"):
+        O.clip_grads_([g], 1.0)
