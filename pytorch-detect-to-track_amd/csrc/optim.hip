@@ -195,8 +195,9 @@ template <typename T, int N> __device__ __forceinline__ void scale_run(T* g, lon
   for (; e < e1; ++e) g[e] = (T)((float)g[e] * f);
 }
 
-// Every workgroup joins the partial sums itself (16 KiB of L2 at most): a launch of one workgroup in between would keep the device
-// waiting for 7 us.
+// Every workgroup joins the partial sums itself -- at most 2048 and one per tensor, 8 bytes each: 17 KiB of L2 for Res-101 -- because a
+// launch of one workgroup in between would keep the device waiting for 7 us.  The reading grows with the square of the number of tensors:
+// 10 000 of 500 elements are 10 000 workgroups that read 80 KB each (norm alone 591 us, with the scaling 842; 1000 of them 65 / 94).
 __global__ __launch_bounds__(kThreads) void grad_clip_kernel(ScaleTable tab, NormPart part, float* __restrict__ out) {
   const float2 r = finish_norm<kThreads>(part.partial, part.n, part.max_norm);
   if (out && blockIdx.x == 0 && threadIdx.x == 0) { out[0] = r.x; out[1] = r.y; }
@@ -213,7 +214,8 @@ __global__ __launch_bounds__(kThreads) void grad_clip_kernel(ScaleTable tab, Nor
 // ------------------------------------------------------------------------------------------------ what a step needs per tensor
 // One thread per tensor: t <- t + 1 in the tensor's step counter, and the step's factors in 64 bits, rounded once:
 // keep = 1 - lr * decay, size = lr / (1 - beta1^t), root = 1 / sqrt(1 - beta2^t); for 8-bit moments the key of its rounding terms.
-// Where the call clips, the same workgroup joins the norm's partial sums first (one launch less than a kernel of its own).
+// Where the call clips, the same workgroup joins the norm's partial sums first (one launch less than a kernel of its own); a call of more
+// than kMaxPrepare tensors or kMaxRates rates has several such launches, and each joins them again.
 // The counters live on the device, so a captured step counts on with every replay.
 struct Rate {
   double lr;
@@ -274,9 +276,10 @@ struct Consts {
 
 // m <- beta1 m + (1 - beta1) g;  v <- beta2 v + (1 - beta2) g^2;  p <- keep p - size * m / (root sqrt(v) + eps)
 // The step with 8-bit moments has about as many instructions as it has bytes: EXACT = false takes the quotient from v_sqrt and v_rcp, each
-// good to 2^-24, in place of the exactly rounded sequences (302 M bf16: step and unpacking 985 -> 884 us).  v_sqrt takes a v below 2^-126
-// for 0: beside eps >= 2^-39 / sqrt(1 - beta2), which is 2^-39 root or more, that is below 2^-24 of the denominator.  A smaller eps takes
-// the exact sequences.
+// off by one unit in the last place (2^-23 of the value) at most, and a product, in place of the exactly rounded sequences (302 M bf16: step
+// and unpacking 985 -> 884 us); the tests' bounds count 2^-23 for each.  v_sqrt takes a v below 2^-126 for 0: beside
+// eps >= 2^-39 / sqrt(1 - beta2), which is 2^-39 root or more, that is below 2^-24 of the denominator.  A smaller eps takes the exact
+// sequences, which are built for one block per wave only.
 template <bool EXACT> __device__ __forceinline__ void adamw_element(float& p, float g, float& m, float& v, const Consts& k, const Factors& f) {
   m = m * k.beta1 + g * k.one_beta1;
   v = v * k.beta2 + (g * g) * k.one_beta2;

@@ -378,8 +378,8 @@ def adamw8_(params, grads, exp_avgs, exp_avg_sqs, bases, steps, *, lr, betas=(0.
     (blocks_of(numel), 2); all zero = moments of zero.  A value has three bits of mantissa; codes span 15.7 (m) and 31.7 (v) powers of
     two below the largest of their block of 256, what lies lower is 0 (m) or the smallest step (v): an element whose gradients stay
     2^-15.7 below its block's largest is not moved.  The rounding of a moment is dithered, right on average, by a hash of seed, ids
-    (default: the position in the list), step counter and element; the same inputs give the same codes.  Infinite and NaN moments stay
-    in their element, as NaN."""
+    (default: the position in the list), step counter and element; the same inputs give the same codes.  Infinite and NaN moments, and
+    those that round beyond the largest float32, stay in their element, as NaN."""
     return _step("adamw8_", [([params, grads, steps, exp_avgs, exp_avg_sqs, bases], lr, betas, eps, weight_decay, ids)], _UINT8, max_norm,
                  skip_nonfinite, clip, seed)
 
