@@ -532,8 +532,9 @@ class GroupedAdamW(torch.optim.Optimizer):
         """The names of a parameter's moments in a checkpoint; raises where the entry is not a state of this parameter."""
         if "step" not in src or not any(all(k in src for k in names) for names in (_MOMENTS32, _MOMENTS8)):
             raise ValueError("GroupedAdamW: not a state of AdamW or Adam (it holds %s)" % sorted(src))
-        if torch.as_tensor(src["step"]).numel() != 1:
-            raise ValueError("GroupedAdamW: step is one number (the checkpoint has shape %s)" % (tuple(src["step"].shape),))
+        step = torch.as_tensor(src["step"])
+        if step.numel() != 1:
+            raise ValueError("GroupedAdamW: step is one number (the checkpoint has shape %s)" % (tuple(step.shape),))
         names = _MOMENTS32 if all(k in src for k in _MOMENTS32) else _MOMENTS8
         m, v = (src[k] for k in names[:2])
         if m.shape != p.shape or v.shape != p.shape:
