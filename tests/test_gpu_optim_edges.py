@@ -141,3 +141,51 @@ def test_negated_views_are_read_as_what_they_are_or_refused():
         x.grad, y.grad = (torch._neg_view(g.clone()), g.clone()) if x is w2 else (-g, g.clone())
         GroupedAdamW([{"params": [x]}, {"params": [y], "betas": (0.8, 0.9)}], lr=0.1, max_norm=1.0).step()
     assert torch.equal(w2, u2) and torch.equal(w3, u3)
+
+
+# ------------------------------------------------------------------------------------------------ captured
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_captured_step_over_types_and_betas_equals_eager_ones(bits):
+    """Three calls under one norm in one graph, a rate in device memory shared by the groups, one gradient in another memory order."""
+    from dtt.optim import GroupedAdamW
+
+    def build():
+        torch.manual_seed(3)
+        ps = [torch.nn.Parameter(torch.randn(*s, device=DEV).to(t)) for s, t in
+              (((40, 30), torch.bfloat16), ((300,), torch.float32), ((17, 5), torch.float32))]
+        for p in ps:
+            p.grad = torch.zeros_like(p)
+        ps[0].grad = torch.zeros(30, 40, dtype=torch.bfloat16, device=DEV).t()
+        rate = torch.full((), 1e-2, device=DEV)
+        return ps, rate, GroupedAdamW([{"params": ps[:2]}, {"params": ps[2:], "betas": (0.8, 0.9)}], lr=rate, state_bits=bits, max_norm=1.0,
+                                      skip_nonfinite=True)
+    (ps, rate, opt), (qs, qrate, ref) = build(), build()
+
+    def gradients(seed):
+        torch.manual_seed(seed)
+        for p, q in zip(ps, qs):
+            p.grad.copy_(torch.randn(p.shape, device=DEV))
+            q.grad.copy_(p.grad)
+    gradients(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        opt.step()
+    torch.cuda.current_stream().wait_stream(side)
+    ref.step()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        opt.step()
+    norm = opt.grad_norm
+    for it in range(4):
+        rate.fill_(1e-2 / (1 + it)); qrate.fill_(1e-2 / (1 + it))
+        gradients(10 + it)
+        if it == 2:
+            ps[2].grad[3, 3] = math.nan; qs[2].grad[3, 3] = math.nan        # skipped in all three calls
+        g.replay()
+        ref.step()
+        torch.cuda.synchronize()
+        assert torch.equal(norm.nan_to_num(-1.0), ref.grad_norm.nan_to_num(-1.0)) and math.isnan(float(norm)) == (it == 2)
+        for p, q in zip(ps, qs):
+            assert torch.equal(p, q) and all(torch.equal(opt.state[p][k], ref.state[q][k]) for k in opt.state[p]), it
+            assert float(opt.state[p]["step"]) == 2 + it - (it >= 2)
